@@ -330,6 +330,124 @@ ifx_status ifx_op_sample_u_static(const float *logits_dev, size_t n,
                                   const ifx_sampler *s, float u,
                                   uint32_t *token_dev, void *stream);
 
+/* ----------------- a paged serving step, on the device ------------------ */
+/* No counterparts in the reference (its KvCache holds one sequence of f32
+ * rows, src/model/cache.rs:7-13; its sampler draws for one row on the host).
+ * What a serving loop runs each step over sequences that share a pool of
+ * cache pages: pages and row slots for the rows that arrive, the rows into
+ * the cache, attention over it, the next tokens. All pointers are device
+ * memory of the current device; every call only enqueues work on `stream`
+ * and may be captured into a graph. Counts and indices are int32.
+ *
+ * A page has IFX_PAGE_ROWS rows. Row `pos` of a sequence lies in the page
+ * table[seq * max_pages + pos / 64]; its slot is page * 64 + pos % 64. */
+#define IFX_PAGE_ROWS 64
+#define IFX_PAGES_MAX_SEQS 8192
+
+/* Pages and slots for add[b] new rows behind the lens[b] rows of every
+ * sequence b. Pages come from the end of the free list free_pages[0 ..
+ * n_free[0]) in the order of sequences and positions and are appended to the
+ * sequences' table rows. Outputs: lens_out [n_seqs], n_free_out [1], q_start
+ * [n_seqs + 1] (the sequences' first new rows, and their number), and per
+ * new row slots, positions and seqs [max_tokens] (the last two nullable),
+ * -1 behind the last row. status [1]: 0, or why nothing was taken and every
+ * slot is -1, lens_out = lens, n_free_out = n_free and q_start 0:
+ * 1 too few free pages, 2 a sequence longer than max_pages pages, 3 more
+ * than max_tokens rows. Inputs and outputs do not overlap (lens_out may not
+ * be lens, nor n_free_out n_free: swap them from step to step); free_pages
+ * [n_pages] is not written. At most IFX_PAGES_MAX_SEQS sequences. */
+ifx_status ifx_op_pages_extend(const int32_t *lens, const int32_t *add,
+                               size_t n_seqs, int32_t *table, size_t max_pages,
+                               const int32_t *free_pages, size_t n_pages,
+                               const int32_t *n_free, size_t max_tokens,
+                               int32_t *lens_out, int32_t *n_free_out,
+                               int32_t *q_start, int32_t *slots,
+                               int32_t *positions, int32_t *seqs,
+                               int32_t *status, void *stream);
+/* Sequences with done[b] != 0 give their pages back: appended to the free
+ * list (free_pages[n_free[0] ..), in the order of sequences and positions),
+ * lens_out[b] = 0. The others keep their lengths. The table is not written.
+ * free_pages holds n_pages entries; lens_out and n_free_out do not overlap
+ * lens and n_free. */
+ifx_status ifx_op_pages_release(const int32_t *done, const int32_t *lens,
+                                size_t n_seqs, const int32_t *table,
+                                size_t max_pages, int32_t *free_pages,
+                                size_t n_pages, const int32_t *n_free,
+                                int32_t *lens_out, int32_t *n_free_out,
+                                void *stream);
+
+/* The cache in 4 bits: keys and values of n_kv_heads heads of head_dim (a
+ * multiple of 32, at most 256) values, each row's blocks of 32 values
+ * quantised as Q4_0 (4.5 bits a value; a NaN counts as 0, and a block's
+ * scale stops at f16's largest value). Bytes of one page; 0 when the shape
+ * is not supported. Pages are 16-byte aligned and may start with any
+ * contents: rows that were never stored are not read as long as kv_len does
+ * not cover them. */
+size_t ifx_kv4_page_bytes(size_t n_kv_heads, size_t head_dim);
+/* Rows i of k and v ([n] rows of n_kv_heads * head_dim values of `type`
+ * IFX_TYPE_F32 or IFX_TYPE_F16, k_stride / v_stride values apart, rows and
+ * base 16-byte aligned) into the rows slots[i] of the pages. A negative slot
+ * or one behind the last page skips the row. The slots of one call differ
+ * from one another (a slot given twice ends as a mixture of both rows). */
+ifx_status ifx_op_kv4_store(int type, const void *k, size_t k_stride,
+                            const void *v, size_t v_stride,
+                            const int32_t *slots, size_t n, void *pages,
+                            size_t n_pages, size_t n_kv_heads, size_t head_dim,
+                            void *stream);
+/* The values that the rows slots[i] stand for, into contiguous k and v
+ * [n, n_kv_heads, head_dim] of `type`; zeros for a slot outside the pages. */
+ifx_status ifx_op_kv4_load(int type, const void *pages, size_t n_pages,
+                           size_t n_kv_heads, size_t head_dim,
+                           const int32_t *slots, size_t n, void *k, void *v,
+                           void *stream);
+/* Causal attention of q [rows, n_heads, head_dim] (`type` IFX_TYPE_F32 or
+ * IFX_TYPE_F16, rows q_stride values apart) over the cache, into out (same
+ * type, out_stride apart; out may not overlap q). Query head i reads kv head
+ * i / (n_heads / n_kv_heads). Sequence b's kv_len[b] rows are in the cache,
+ * the query rows' own among them; its query rows are q_start[b] ..
+ * q_start[b + 1] - 1 (q_start [n_seqs + 1], rising from 0), or row b when
+ * q_start is NULL (rows = n_seqs, one row per sequence). The last query row
+ * sees all kv_len rows, the one before it one less, and so on; with
+ * window > 0 each sees its last `window` rows only. softmax(scale q k) v in
+ * f32 throughout; a row that sees nothing (kv_len 0, or a query row before
+ * the cache's first) gives 0, and rows of out behind the last sequence's are
+ * left as they were. A table entry outside the pages hides its rows.
+ * ws: scratch of at least ifx_kv4_attention_workspace bytes, 256-byte
+ * aligned, any contents, for one call at a time. */
+size_t ifx_kv4_attention_workspace(size_t n_heads, size_t n_kv_heads,
+                                   size_t head_dim);
+ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride,
+                                size_t rows, const void *pages, size_t n_pages,
+                                const int32_t *table, size_t max_pages,
+                                const int32_t *kv_len, const int32_t *q_start,
+                                size_t n_seqs, size_t n_heads,
+                                size_t n_kv_heads, size_t head_dim, float scale,
+                                size_t window, void *out, size_t out_stride,
+                                void *ws, size_t ws_bytes, void *stream);
+
+/* The next token of every row of logits [rows, n] (rows `stride` values
+ * apart, n at most IFX_SAMPLE_ROWS_MAX): Sampler::sample's rule
+ * (src/sampler.rs:28-73) with each row's own settings and given u [rows] in
+ * [0, 1), and min-p beside its filters. With w_i = exp((z_i - max z) / T),
+ * tokens are ordered by falling z and, among equal ones, rising index; kept
+ * are the first top_k[r] (0: all), of these the first whose masses reach
+ * top_p[r] of the whole row's mass (1: all), and of these the ones with
+ * w_i >= min_p[r] (0: all). Drawn is the first kept token at which the kept
+ * mass so far exceeds u[r] of the kept mass; when no filter is on, in index
+ * order. temperature[r] <= 0 takes the largest logit (the last index among
+ * equal ones, as argmax). NaN counts as minus infinity, a masked token; a
+ * row without any other gives token -1 and logprob -inf. NULL settings:
+ * temperature 1, no filter. logprob (nullable): the logarithm of the drawn
+ * token's share of the kept mass (0 when greedy). Masses are summed as
+ * 64-bit integers (weights to 2^-45 at 128k tokens, 2^-61 at one), so the
+ * result does not depend on the order of additions. */
+#define IFX_SAMPLE_ROWS_MAX (1 << 24)
+ifx_status ifx_op_sample_rows(const float *logits, size_t stride, size_t rows,
+                              size_t n, const float *u,
+                              const float *temperature, const int32_t *top_k,
+                              const float *top_p, const float *min_p,
+                              int32_t *token, float *logprob, void *stream);
+
 /* ------------------------- tensor parallelism --------------------------- */
 /* No reference counterpart (the reference is single-threaded CPU code).
  * Megatron split across tp_size GPUs of one box: Wq/Wk/Wv, W1/W3 and the

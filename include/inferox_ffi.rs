@@ -116,6 +116,37 @@ extern "C" {
                            token_host: *mut u32, stream: *mut c_void) -> c_int;
     pub fn ifx_op_sample_u_static(logits: *const f32, n: usize, s: *const IfxSampler, u: f32,
                                   token_dev: *mut u32, stream: *mut c_void) -> c_int;
+    // a paged serving step: device pointers, work enqueued on `stream`
+    pub fn ifx_op_pages_extend(lens: *const i32, add: *const i32, n_seqs: usize, table: *mut i32,
+                               max_pages: usize, free_pages: *const i32, n_pages: usize,
+                               n_free: *const i32, max_tokens: usize, lens_out: *mut i32,
+                               n_free_out: *mut i32, q_start: *mut i32, slots: *mut i32,
+                               positions: *mut i32, seqs: *mut i32, status: *mut i32,
+                               stream: *mut c_void) -> c_int;
+    pub fn ifx_op_pages_release(done: *const i32, lens: *const i32, n_seqs: usize,
+                                table: *const i32, max_pages: usize, free_pages: *mut i32,
+                                n_pages: usize, n_free: *const i32, lens_out: *mut i32,
+                                n_free_out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ifx_kv4_page_bytes(n_kv_heads: usize, head_dim: usize) -> usize;
+    pub fn ifx_op_kv4_store(ty: c_int, k: *const c_void, k_stride: usize, v: *const c_void,
+                            v_stride: usize, slots: *const i32, n: usize, pages: *mut c_void,
+                            n_pages: usize, n_kv_heads: usize, head_dim: usize,
+                            stream: *mut c_void) -> c_int;
+    pub fn ifx_op_kv4_load(ty: c_int, pages: *const c_void, n_pages: usize, n_kv_heads: usize,
+                           head_dim: usize, slots: *const i32, n: usize, k: *mut c_void,
+                           v: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ifx_kv4_attention_workspace(n_heads: usize, n_kv_heads: usize, head_dim: usize) -> usize;
+    pub fn ifx_op_kv4_attention(ty: c_int, q: *const c_void, q_stride: usize, rows: usize,
+                                pages: *const c_void, n_pages: usize, table: *const i32,
+                                max_pages: usize, kv_len: *const i32, q_start: *const i32,
+                                n_seqs: usize, n_heads: usize, n_kv_heads: usize,
+                                head_dim: usize, scale: f32, window: usize, out: *mut c_void,
+                                out_stride: usize, ws: *mut c_void, ws_bytes: usize,
+                                stream: *mut c_void) -> c_int;
+    pub fn ifx_op_sample_rows(logits: *const f32, stride: usize, rows: usize, n: usize,
+                              u: *const f32, temperature: *const f32, top_k: *const i32,
+                              top_p: *const f32, min_p: *const f32, token: *mut i32,
+                              logprob: *mut f32, stream: *mut c_void) -> c_int;
     // tensor parallelism: a communicator made by the library's own NCCL instance
     pub fn ifx_tp_unique_id(id_out: *mut u8) -> c_int;  // 128 bytes, on rank 0
     pub fn ifx_tp_comm_create(id: *const u8, nranks: c_int, rank: c_int, device: c_int,

@@ -136,6 +136,15 @@ def _load():
         "ifx_op_argmax": (st, [vp, sz, vp, vp]),
         "ifx_op_sample_u": (st, [vp, sz, C.POINTER(SamplerC), C.c_float, u32p, vp]),
         "ifx_op_sample_u_static": (st, [vp, sz, C.POINTER(SamplerC), C.c_float, vp, vp]),
+        "ifx_op_pages_extend": (st, [vp, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "ifx_op_pages_release": (st, [vp, vp, sz, vp, sz, vp, sz, vp, vp, vp, vp]),
+        "ifx_kv4_page_bytes": (sz, [sz, sz]),
+        "ifx_op_kv4_store": (st, [C.c_int, vp, sz, vp, sz, vp, sz, vp, sz, sz, sz, vp]),
+        "ifx_op_kv4_load": (st, [C.c_int, vp, sz, sz, sz, vp, sz, vp, vp, vp]),
+        "ifx_kv4_attention_workspace": (sz, [sz, sz, sz]),
+        "ifx_op_kv4_attention": (st, [C.c_int, vp, sz, sz, vp, sz, vp, sz, vp, vp, sz, sz, sz, sz,
+                                      C.c_float, sz, vp, sz, vp, sz, vp]),
+        "ifx_op_sample_rows": (st, [vp, sz, sz, sz, vp, vp, vp, vp, vp, vp, vp, vp]),
         "ifx_kquant_from_ggml": (st, [C.c_uint32, vp, sz, vp, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
         "ifx_tokenizer_load": (st, [C.c_char_p, C.POINTER(vp)]),
         "ifx_tokenizer_load_json": (st, [C.c_char_p, sz, C.POINTER(vp)]),

@@ -7,6 +7,7 @@ Shape mismatches raise IfxError("Shape") where the reference panics.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -152,3 +153,217 @@ def sample_u(logits, temperature, top_k, top_p, u) -> int:
     check(lib.ifx_op_sample_u(_p(logits), logits.numel(), C.byref(s), float(u), C.byref(tok),
                               _s()), "sample_u")
     return int(tok.value)
+
+
+# ---- a paged serving step on the device (no counterparts in the reference) --
+PAGE_ROWS = 64
+_TYPES = {torch.float32: 0, torch.float16: 1}
+
+
+def _dev(*tensors) -> int:
+    """The one CUDA device the tensors are on."""
+    d = tensors[0].device
+    for t in tensors:
+        if t.device != d or not t.is_cuda:
+            raise IfxError(24, "expected CUDA tensors of one device")
+    return d.index
+
+
+def _ints(what: str, *tensors):
+    for t in tensors:
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise IfxError(24, f"{what}: expected contiguous int32 tensors")
+
+
+def _call(dev: int, what: str, fn, *args):
+    """fn(*args, stream) on the current stream of device `dev`."""
+    if dev == torch.cuda.current_device():
+        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if code:
+        check(code, what)
+
+
+class PageStep(NamedTuple):
+    """What pages_extend gives: the sequences' new lengths, the free list's new
+    length, the sequences' first new rows [n_seqs + 1], each new row's slot,
+    position and sequence [max_tokens] (-1 behind the last), and the status
+    (0, or 1 too few free pages, 2 a sequence beyond its table row, 3 more
+    rows than max_tokens: nothing was taken)."""
+
+    lens: torch.Tensor
+    n_free: torch.Tensor
+    q_start: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    seqs: torch.Tensor
+    status: torch.Tensor
+
+
+def pages_extend(lens, add, table, free, n_free, max_tokens: int) -> PageStep:
+    """Pages and slots for add[b] new rows behind sequence b's lens[b] rows.
+    table [n_seqs, max_pages] takes the new pages, from the end of
+    free[:n_free]; all int32. The caller goes on with the returned lens and
+    n_free. Nothing is copied to the host: the status is on the device."""
+    dev = _dev(lens, add, table, free, n_free)
+    _ints("pages_extend", lens, add, table, free, n_free)
+    n = lens.numel()
+    _need(table.dim() == 2 and table.shape[0] == n and add.numel() == n and n_free.numel() == 1,
+          "pages_extend shape mismatch")
+    _need(max_tokens >= 0, "pages_extend: negative max_tokens")
+    # one allocation, its parts 16-byte aligned
+    m4, n4 = (max_tokens + 3) & ~3, (n + 4) & ~3
+    buf = torch.empty(3 * m4 + 2 * n4 + 8, dtype=torch.int32, device=lens.device)
+    p = buf.data_ptr()
+    lo, qs, nf, sl = 3 * m4, 3 * m4 + n4, 3 * m4 + 2 * n4, 3 * m4 + 2 * n4 + 4
+    _call(dev, "pages_extend", lib.ifx_op_pages_extend, lens.data_ptr(), add.data_ptr(), n, table.data_ptr(),
+          table.shape[1], free.data_ptr(), free.numel(), n_free.data_ptr(), max_tokens, p + 4 * lo, p + 4 * nf,
+          p + 4 * qs, p, p + 4 * m4, p + 8 * m4, p + 4 * sl)
+    return PageStep(buf[lo:lo + n], buf[nf:nf + 1], buf[qs:qs + n + 1], buf[:max_tokens],
+                    buf[m4:m4 + max_tokens], buf[2 * m4:2 * m4 + max_tokens], buf[sl:sl + 1])
+
+
+def pages_release(done, lens, table, free, n_free):
+    """Sequences with done[b] != 0 give their pages back to the end of
+    free[:n_free]; returns (lens, n_free) to go on with."""
+    dev = _dev(done, lens, table, free, n_free)
+    _ints("pages_release", done, lens, table, free, n_free)
+    n = lens.numel()
+    _need(table.dim() == 2 and table.shape[0] == n and done.numel() == n and n_free.numel() == 1,
+          "pages_release shape mismatch")
+    lens_out, n_free_out = torch.empty_like(lens), torch.empty_like(n_free)
+    _call(dev, "pages_release", lib.ifx_op_pages_release, done.data_ptr(), lens.data_ptr(), n, table.data_ptr(),
+          table.shape[1], free.data_ptr(), free.numel(), n_free.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr())
+    return lens_out, n_free_out
+
+
+def kv4_page_bytes(n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of one page (64 rows of keys and values) of the cache in 4 bits."""
+    n = lib.ifx_kv4_page_bytes(n_kv_heads, head_dim)
+    if not n:
+        raise IfxError(26, "kv4: 1 to 1024 kv heads, head_dim a multiple of 32 up to 256")
+    return n
+
+
+def kv4_pages(n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Memory for n_pages pages, uint8 [n_pages, page bytes]."""
+    return torch.zeros(n_pages, kv4_page_bytes(n_kv_heads, head_dim), dtype=torch.uint8, device=device)
+
+
+def _pool(what: str, pages: torch.Tensor, n_kv_heads: int, head_dim: int) -> int:
+    if pages.dtype != torch.uint8 or pages.dim() != 2 or not pages.is_contiguous():
+        raise IfxError(24, f"{what}: pages must be a contiguous uint8 tensor [n_pages, page bytes]")
+    _need(pages.shape[1] == kv4_page_bytes(n_kv_heads, head_dim), f"{what}: page bytes mismatch")
+    return pages.shape[0]
+
+
+def _rows(what: str, x: torch.Tensor) -> int:
+    """Stride between the rows of x [n, heads, head_dim], whose rows are contiguous."""
+    if x.dtype not in _TYPES:
+        raise IfxError(26, f"{what}: float32 or float16 rows")
+    _need(x.dim() == 3, f"{what}: expected [rows, heads, head_dim]")
+    n, h, d = x.shape
+    if not x.numel():
+        return h * d
+    sn, sh, sd = x.stride()
+    if (sd != 1 and d != 1) or (sh != d and h != 1):
+        raise IfxError(24, f"{what}: a row's heads must be contiguous")
+    return sn if n > 1 else h * d
+
+
+def kv4_store(k, v, slots, pages) -> None:
+    """Rows k, v [n, n_kv_heads, head_dim] quantised into the rows slots [n] of
+    the pages; a slot outside them (-1) skips its row. The slots differ."""
+    dev = _dev(k, v, slots, pages)
+    ks, vs = _rows("kv4_store", k), _rows("kv4_store", v)
+    _need(k.shape == v.shape and k.dtype == v.dtype and slots.numel() == k.shape[0], "kv4_store shape mismatch")
+    _ints("kv4_store", slots)
+    n, g, d = k.shape
+    np_ = _pool("kv4_store", pages, g, d)
+    _call(dev, "kv4_store", lib.ifx_op_kv4_store, _TYPES[k.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
+          slots.data_ptr(), n, pages.data_ptr(), np_, g, d)
+
+
+def kv4_load(slots, pages, n_kv_heads: int, head_dim: int, dtype=torch.float32):
+    """The values of the rows slots [n]: (k, v) [n, n_kv_heads, head_dim]; zeros
+    for a slot outside the pages."""
+    dev = _dev(slots, pages)
+    _ints("kv4_load", slots)
+    np_ = _pool("kv4_load", pages, n_kv_heads, head_dim)
+    if dtype not in _TYPES:
+        raise IfxError(26, "kv4_load: float32 or float16 rows")
+    n = slots.numel()
+    k = torch.empty(n, n_kv_heads, head_dim, dtype=dtype, device=slots.device)
+    v = torch.empty_like(k)
+    _call(dev, "kv4_load", lib.ifx_op_kv4_load, _TYPES[dtype], pages.data_ptr(), np_, n_kv_heads, head_dim,
+          slots.data_ptr(), n, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def kv4_attention(q, pages, table, kv_len, n_kv_heads: int, q_start=None, scale=None, window: int = 0,
+                  out=None, workspace=None) -> torch.Tensor:
+    """Causal attention of q [rows, n_heads, head_dim] over the cache in 4 bits.
+    Sequence b has kv_len[b] rows in the cache, the query rows' own among
+    them, in the pages table[b]; its query rows are q_start[b]:q_start[b + 1],
+    or row b when q_start is None. scale: 1 / sqrt(head_dim) when None;
+    window > 0: each row sees its last `window` rows. A row that sees nothing
+    gives 0; rows of `out` behind the last sequence's stay as they were (a
+    fresh `out` is zeroed when q_start is given). workspace: uint8 scratch kept
+    by the caller (kv4_workspace), for one call at a time."""
+    qs = _rows("kv4_attention", q)
+    rows, h, d = q.shape
+    n = kv_len.numel()
+    _need(n_kv_heads > 0 and h % n_kv_heads == 0, "kv4_attention: query heads must be a multiple of the kv heads")
+    np_ = _pool("kv4_attention", pages, n_kv_heads, d)
+    _ints("kv4_attention", table, kv_len)
+    _need(table.dim() == 2 and table.shape[0] == n, "kv4_attention: table is [n_seqs, max_pages]")
+    _need(window >= 0, "kv4_attention: negative window")
+    if q_start is None:
+        _need(rows == n, "kv4_attention: one row per sequence without q_start")
+    else:
+        _ints("kv4_attention", q_start)
+        _need(q_start.numel() == n + 1, "kv4_attention: q_start is [n_seqs + 1]")
+    if out is None:
+        out = (torch.empty if q_start is None else torch.zeros)(rows, h, d, dtype=q.dtype, device=q.device)
+    _need(out.shape == q.shape and out.dtype == q.dtype, "kv4_attention: out mismatch")
+    if workspace is None:
+        workspace = kv4_workspace(h, n_kv_heads, d, q.device)
+    dev = _dev(q, pages, table, kv_len, out, workspace, *(() if q_start is None else (q_start,)))
+    _call(dev, "kv4_attention", lib.ifx_op_kv4_attention, _TYPES[q.dtype], q.data_ptr(), qs, rows, pages.data_ptr(),
+          np_, table.data_ptr(), table.shape[1], kv_len.data_ptr(), None if q_start is None else q_start.data_ptr(),
+          n, h, n_kv_heads, d, d ** -0.5 if scale is None else scale, window, out.data_ptr(),
+          _rows("kv4_attention", out), workspace.data_ptr(), workspace.numel())
+    return out
+
+
+def kv4_workspace(n_heads: int, n_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Scratch of kv4_attention for these shapes."""
+    return torch.empty(lib.ifx_kv4_attention_workspace(n_heads, n_kv_heads, head_dim), dtype=torch.uint8, device=device)
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of every row of logits [rows, n] (float32), by
+    Sampler::sample's rule with min-p beside its filters and the uniform draws
+    u [rows] given: (tokens int32 [rows], logprobs float32 [rows]). Settings
+    are tensors [rows] or one value for all rows. temperature <= 0 is greedy;
+    a row whose logits are all masked (-inf, NaN) gives token -1."""
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise IfxError(24, "sample_rows: logits must be float32 [rows, n] with contiguous rows")
+    rows, n = logits.shape
+    at = []
+    for x, dt in ((u, torch.float32), (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32),
+                  (min_p, torch.float32)):
+        if not isinstance(x, torch.Tensor):
+            x = torch.full((rows,), x, dtype=dt, device=logits.device)
+        if x.dtype != dt or not x.is_contiguous():
+            raise IfxError(24, "sample_rows: settings are contiguous float32 tensors, top_k int32")
+        _need(x.numel() == rows, "sample_rows shape mismatch")
+        at.append(x)
+    dev = _dev(logits, *at)
+    token = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    logp = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    _call(dev, "sample_rows", lib.ifx_op_sample_rows, logits.data_ptr(), logits.stride(0) if rows > 1 else n, rows, n,
+          *(x.data_ptr() for x in at), token.data_ptr(), logp.data_ptr())
+    return token, logp
