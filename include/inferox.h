@@ -343,6 +343,7 @@ ifx_status ifx_op_sample_u_static(const float *logits_dev, size_t n,
  * table[seq * max_pages + pos / 64]; its slot is page * 64 + pos % 64. */
 #define IFX_PAGE_ROWS 64
 #define IFX_PAGES_MAX_SEQS 8192
+#define IFX_KV4_ATTENTION_MAX_SEQS 2048
 
 /* Pages and slots for add[b] new rows behind the lens[b] rows of every
  * sequence b. Pages come from the end of the free list free_pages[0 ..
@@ -411,7 +412,8 @@ ifx_status ifx_op_kv4_load(int type, const void *pages, size_t n_pages,
  * window > 0 each sees its last `window` rows only. softmax(scale q k) v in
  * f32 throughout; a row that sees nothing (kv_len 0, or a query row before
  * the cache's first) gives 0, and rows of out behind the last sequence's are
- * left as they were. A table entry outside the pages hides its rows.
+ * left as they were. A table entry outside the pages hides its rows. At most
+ * IFX_KV4_ATTENTION_MAX_SEQS sequences.
  * ws: scratch of at least ifx_kv4_attention_workspace bytes, 256-byte
  * aligned, any contents, for one call at a time. */
 size_t ifx_kv4_attention_workspace(size_t n_heads, size_t n_kv_heads,

@@ -7,7 +7,8 @@ namespace ifx {
 
 constexpr int kKv4PageRows = 64;  // rows of a page
 constexpr int kKv4TileRows = 16;  // rows of a tile (four tiles per page and kv head)
-constexpr int kMaxServeSeqs = 8192;
+constexpr int kMaxServeSeqs = 8192;  // pages_extend / pages_release
+constexpr int kMaxAttnSeqs = 2048;   // kv4_attention: their running totals stay in shared memory
 
 // The 4-bit cache (no reference counterpart; its KvCache holds f32 rows,
 // src/model/cache.rs:7-14). A page holds 64 rows; for each kv head four

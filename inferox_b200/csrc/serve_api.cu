@@ -17,10 +17,9 @@ ifx_status bad(const char *what) { return fail(IFX_ERR_INVALID_ARGUMENT, what); 
 constexpr size_t kIntMax = 0x7fffffff;
 constexpr size_t kMaxPoolPages = kIntMax / kKv4PageRows;  // slots are int32
 
-ifx_status check_pool(size_t n_seqs, size_t max_pages, size_t n_pages, const char *name) {
+ifx_status check_pool(size_t n_seqs, size_t most, size_t max_pages, size_t n_pages, const char *name) {
   const std::string n(name);
-  if (n_seqs > (size_t)kMaxServeSeqs)
-    return fail(IFX_ERR_INVALID_ARGUMENT, n + ": more than " + std::to_string(kMaxServeSeqs) + " sequences");
+  if (n_seqs > most) return fail(IFX_ERR_INVALID_ARGUMENT, n + ": more than " + std::to_string(most) + " sequences");
   if (max_pages > kMaxPoolPages || n_pages > kMaxPoolPages)
     return fail(IFX_ERR_INVALID_ARGUMENT, n + ": too many pages for 32-bit slots");
   return IFX_OK;
@@ -53,7 +52,7 @@ ifx_status ifx_op_pages_extend(const int32_t *lens, const int32_t *add, size_t n
     return bad("pages_extend: null");
   if (lens_out == lens && n_seqs) return bad("pages_extend: lens_out is lens");
   if (n_free_out == n_free) return bad("pages_extend: n_free_out is n_free");
-  IFX_TRY(check_pool(n_seqs, max_pages, n_pages, "pages_extend"));
+  IFX_TRY(check_pool(n_seqs, kMaxServeSeqs, max_pages, n_pages, "pages_extend"));
   if (max_tokens > kIntMax) return bad("pages_extend: max_tokens above 2^31 - 1");
   PagesExtendArgs a{lens, add, (int)n_seqs, table, (int)max_pages, free_pages, (int)n_pages, n_free,
                     (int64_t)max_tokens, lens_out, n_free_out, q_start, slots, positions, seqs, status};
@@ -68,7 +67,7 @@ ifx_status ifx_op_pages_release(const int32_t *done, const int32_t *lens, size_t
     return bad("pages_release: null");
   if (lens_out == lens && n_seqs) return bad("pages_release: lens_out is lens");
   if (n_free_out == n_free) return bad("pages_release: n_free_out is n_free");
-  IFX_TRY(check_pool(n_seqs, max_pages, n_pages, "pages_release"));
+  IFX_TRY(check_pool(n_seqs, kMaxServeSeqs, max_pages, n_pages, "pages_release"));
   PagesReleaseArgs a{done, lens, (int)n_seqs, table, (int)max_pages, free_pages, (int)n_pages, n_free, lens_out, n_free_out};
   return op_pages_release(a, S(stream));
 }
@@ -127,8 +126,8 @@ ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride, size_t
   if (q_stride < w || out_stride < w) return fail(IFX_ERR_SHAPE, "kv4_attention: rows overlap");
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(pages, 16) || q_stride * ts % 16 || out_stride * ts % 16)
     return bad("kv4_attention: rows and pages must be 16-byte aligned");
-  IFX_TRY(check_pool(n_seqs, max_pages, n_pages, "kv4_attention"));
-  if (rows > kIntMax || rows * n_heads > (size_t)kIntMax * 4) return bad("kv4_attention: too many rows");
+  IFX_TRY(check_pool(n_seqs, kMaxAttnSeqs, max_pages, n_pages, "kv4_attention"));
+  if (rows > kIntMax || rows * n_heads > kIntMax) return bad("kv4_attention: too many rows");
   if (!(scale == scale) || scale - scale != 0.f) return bad("kv4_attention: scale is not finite");
   if (ws_bytes < kv4_attention_ws((int)n_heads, (int)n_kv_heads, (int)head_dim) || (ws_bytes && (!ws || !aligned(ws, 256))))
     return bad("kv4_attention: workspace too small or not 256-byte aligned");
