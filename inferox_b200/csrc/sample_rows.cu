@@ -7,16 +7,18 @@
 // order of additions and a draw is the same in every layout. Nothing is
 // sorted as a whole: in the order of falling z the kept tokens are a prefix,
 // and the cut and the draw are each a place where a running count or mass
-// passes a target. Such a place is found by a histogram over 2048 buckets of
-// equal width in z (the last one takes all tokens whose weight rounds to 0),
-// a gather of the bucket (or, when they are few, of all buckets up to it)
-// and a sort of what was gathered.
+// passes a target. Tokens are counted in 2048 buckets of equal width in z
+// (the last one takes all whose weight rounds to 0). A bucket is so narrow
+// that its count times the weight of its middle is its mass to 1%: that
+// guesses the place, and one pass that sums the masses before a window of 64
+// buckets and of each bucket in it makes it exact. The bucket (or, when they
+// are few, all up to it) is gathered and sorted.
 //
 // What bounds it. A row is read once (4 n bytes) into the shared memory of a
 // cluster of CTAs, which keeps it for the passes that follow; the weights
-// cost about 20 instructions in 64-bit floating point each, which overlap
-// the reads of other rows. One row alone is bound by latency: five to seven
-// cluster barriers.
+// cost about 20 instructions each, 13 of them in 64-bit floating point (an
+// SM does two warps' worth a clock), which overlap the reads of other rows.
+// One row alone is bound by latency: a cluster barrier takes 1 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -34,6 +36,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512;
 constexpr int kBuckets = 2048;
 constexpr int kList = 2048;      // elements a gather can hold
+constexpr int kWindow = 64;      // buckets whose masses one pass makes exact
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunk = 36864; // elements of a row that one CTA keeps in shared memory
 
@@ -45,6 +48,16 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+
+__device__ const double kPow2[32] = {  // 2^(j / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 
 struct Row {
   float zmax;
@@ -58,9 +71,7 @@ struct Row {
 // / T = 32 n + j + f, |f| <= 1/2, it is 2^n 2^(j/32) e^y, y = f ln2 / 32. Five
 // terms of the series leave y^6 / 720 < 2^-48.
 __device__ __forceinline__ double weight(const Row &r, float z) {
-  if (z == r.zmax) return 1.0;
   const double d = (double)z - (double)r.zmax;
-  if (!(-d < r.cut)) return 0.0;
   const double x = d * r.c;
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
   const double k = x + kRound, f = x - (k - kRound);
@@ -68,7 +79,8 @@ __device__ __forceinline__ double weight(const Row &r, float z) {
   const double e = fma(f, fma(f, fma(f, fma(f, fma(f, y5, y4), y3), y2), y1), 1.0);
   const int i = __double2loint(k);
   const double t = r.pow2[i & 31] * e;
-  return __hiloint2double(__double2hiint(t) + (i >> 5) * (1 << 20), __double2loint(t));
+  const double w = __hiloint2double(__double2hiint(t) + (i >> 5) * (1 << 20), __double2loint(t));
+  return z == r.zmax ? 1.0 : -d < r.cut ? w : 0.0;
 }
 __device__ __forceinline__ u64 to_mass(const Row &r, double w) {
   // w 2^s <= 2^50: adding 2^52 leaves the rounded integer in the low bits
@@ -80,15 +92,16 @@ struct Shared {
   double pow2[32];
   u64 red[kThreads / 32];
   u64 best;            // this CTA's largest value and its last index
-  u64 mass;            // this CTA's total mass
+  u64 mass;            // this CTA's mass: of all its tokens, or before the window
+  u64 window[kWindow]; // ... and of each bucket in it
   u64 pick;
   int count, listed;   // tokens with w >= min_p; length of the list
   float zmax;
   int last;
   // the leader's orders to the cluster
-  int cmd, level, b0, lo, hi;
+  int cmd, level, b0, lo, hi, masses;
 };
-enum { kDone, kHist, kGather };
+enum { kDone, kHist, kMass, kGather };
 
 __device__ __forceinline__ u64 block_sum(u64 v, Shared &sh) {
 #pragma unroll
@@ -103,18 +116,30 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared &sh) {
 }
 // Sum of the lower threads' values.
 __device__ __forceinline__ u64 block_before(u64 v, Shared &sh) {
+  const int lane = threadIdx.x & 31;
   u64 inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 x = __shfl_up_sync(0xffffffffu, inc, o);
-    if ((threadIdx.x & 31) >= o) inc += x;
+    if (lane >= o) inc += x;
   }
   __syncthreads();
-  if ((threadIdx.x & 31) == 31) sh.red[threadIdx.x >> 5] = inc;
+  if (lane == 31) sh.red[threadIdx.x >> 5] = inc;
   __syncthreads();
   u64 base = inc - v;
-  for (int i = 0; i < (int)(threadIdx.x >> 5); ++i) base += sh.red[i];
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) base += i < (int)(threadIdx.x >> 5) ? sh.red[i] : 0;
   return base;
+}
+__device__ __forceinline__ int block_min(int v, Shared &sh) {
+  v = __reduce_min_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.red[threadIdx.x >> 5] = (u64)v;
+  __syncthreads();
+  int m = (int)sh.red[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) m = min(m, (int)sh.red[i]);
+  return m;
 }
 
 // ------------------------------------------------------- the long way round
@@ -205,7 +230,7 @@ __device__ int long_way(const Row &r, const float *z, int n, u64 k_eff, u64 p_ma
 // stays in its shared memory; otherwise every pass reads it from global
 // memory (rows beyond 8 * kMaxChunk tokens).
 template <bool IN_SMEM>
-__global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a) {
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -213,12 +238,13 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
   const int64_t row = blockIdx.y;
   const int n = (int)a.n, per = ((n + C - 1) / C + 3) & ~3, lo = min(n, rank * per), len = min(n, lo + per) - lo;
   const float *zrow = a.logits + row * a.stride;
-  u64 *hmass = reinterpret_cast<u64 *>(sm);                       // [kBuckets]
-  int *hcount = reinterpret_cast<int *>(hmass + kBuckets);        // [kBuckets]
-  u64 *list = reinterpret_cast<u64 *>(hcount + kBuckets);         // [kList], the leader's
-  float *zs = reinterpret_cast<float *>(list + kList);            // [per]
+  u64 *list = reinterpret_cast<u64 *>(sm);                        // [kList], the leader's
+  u64 *guess = list + kList;                                      // [kBuckets], the leader's
+  int *hcount = reinterpret_cast<int *>(guess + kBuckets);        // [kBuckets]
+  float *zs = reinterpret_cast<float *>(hcount + kBuckets);       // [per]
   auto value = [&](int i) { return IN_SMEM ? zs[i] : clean(zrow[lo + i]); };
 
+  if (tid < 32) sh.pow2[tid] = kPow2[tid];
   // ---- read the row; its largest value and the last index that has it
   float top = -INFINITY;
   int at = -1;
@@ -230,6 +256,7 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
   };
   if ((reinterpret_cast<uintptr_t>(zrow) & 15) == 0) {
     const float4 *src = reinterpret_cast<const float4 *>(zrow + lo);
+#pragma unroll 4
     for (int i = tid; i < len / 4; i += kThreads) {
       float4 v = __ldcs(src + i);
       v = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
@@ -252,8 +279,7 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) sh.red[warp] = best;
-  if (tid < 32) sh.pow2[tid] = exp2((double)tid * 0.03125);
-  for (int i = tid; i < kBuckets; i += kThreads) hmass[i] = 0, hcount[i] = 0;
+  for (int i = tid; i < kBuckets; i += kThreads) hcount[i] = 0;
   __syncthreads();
   if (tid == 0) {
     for (int i = 0; i < kThreads / 32; ++i) best = max(best, sh.red[i]);
@@ -309,6 +335,7 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
     // its CTA's share; the one that holds the target walks its run again
     const int run = ((len + kThreads / 32 - 1) / (kThreads / 32) + 31) & ~31, w0 = min(len, warp * run), w1 = min(len, w0 + run);
     u64 m = 0;
+#pragma unroll 4
     for (int i = w0 + lane; i < w1; i += 32) m += to_mass(r, weight(r, value(i)));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
@@ -327,23 +354,23 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
       total += x;
     }
     const u64 target = min((u64)(u * (double)total), total - 1);
-    for (int i = 0; i < warp; ++i) before += sh.red[i];
-    if (before <= target && target < before + m) {
-      for (int i0 = w0; i0 < w1; i0 += 32) {
-        const u64 x = i0 + lane < w1 ? to_mass(r, weight(r, value(i0 + lane))) : 0;
-        u64 inc = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += y;
+    if (before <= target && target < before + sh.mass) {
+      // this CTA: the warp's run that holds the target, two tokens a thread
+      int w = 0;
+      while (w < kThreads / 32 - 1 && before + sh.red[w] <= target) before += sh.red[w++];
+      const int r0 = min(len, w * run), r1 = min(len, r0 + run), each = (r1 - r0 + kThreads - 1) / kThreads;
+      const int e0 = min(r1, r0 + tid * each), e1 = min(r1, e0 + each);
+      u64 mine = 0;
+      for (int i = e0; i < e1; ++i) mine += to_mass(r, weight(r, value(i)));
+      before += block_before(mine, sh);
+      if (before <= target && target < before + mine)
+        for (int i = e0; i < e1; ++i) {
+          before += to_mass(r, weight(r, value(i)));
+          if (before > target) {
+            finish(lo + i, total);
+            break;
+          }
         }
-        const uint32_t over = __ballot_sync(0xffffffffu, before + inc > target);
-        if (over) {
-          if (lane == 0) finish(lo + i0 + __ffs(over) - 1, total);
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, inc, 31);
-      }
     }
     cluster.sync();  // others may still read this CTA's mass
     return;
@@ -352,94 +379,116 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
   // ---- filters
   Shared *boss = cluster.map_shared_rank(&sh, 0);
   u64 *boss_list = cluster.map_shared_rank(list, 0);
-  auto bucket = [&](float z) {
-    const float d = z == r.zmax ? 0.f : r.zmax - z;
-    return min(kBuckets - 1, (int)(d * scale));
+  auto depth = [&](float z) { return z == r.zmax ? 0.f : r.zmax - z; };
+  // the bucket of z, or (level 1) its place among the 2048 parts of bucket
+  // b0; -1: not there. Both rise with falling z.
+  auto bucket = [&](float z, int level, int b0) {
+    const float d = depth(z);
+    const int b = min(kBuckets - 1, (int)(d * scale));
+    if (level == 0) return b;
+    return b == b0 ? min(kBuckets - 1, max(0, (int)(fmaf(d, scale, -(float)b0) * kBuckets))) : -1;
   };
-  auto within_bucket = [&](float z, int b) {  // a bucket's own buckets
-    const float d = z == r.zmax ? 0.f : r.zmax - z;
-    return min(kBuckets - 1, max(0, (int)(fmaf(d, scale, -(float)b) * kBuckets)));
-  };
-  // masses are needed for top-p, and where the cut may leave more than a list
-  bool masses = top_p < 1.f || top_k <= 0 || top_k > kList / 2;
+  int cmd = kHist, level = 0, b0 = 0, glo = 0, ghi = 0;
+  bool masses = top_p < 1.f || top_k <= 0 || top_k > kList / 2 || min_p > 0.f;  // the first pass sums them all
+  bool first = true;
   // the leader's bookkeeping, the same in all its threads
-  u64 total = 0, k_eff = 0, p_mass = 0, kept = 0, target = 0, cbase = 0, mbase = 0;
-  bool drawing = false, first = true;
-  int level = 0, b0 = 0, cmd = kHist, glo = 0, ghi = 0;
+  u64 total = 0, gtotal = 0, k_eff = 0, p_mass = 0, kept = 0, target = 0;
+  u64 cbase = 0, mbase = 0;  // count and mass before what is gathered
+  u64 cup = 0, mup = 0;      // ... before the bucket that level 1 splits
+  bool drawing = false, whole_list = false;
+  int tries = 0;
   for (;;) {
     if (cmd == kHist) {
       if (!first) {
-        for (int i = tid; i < kBuckets; i += kThreads) hmass[i] = 0, hcount[i] = 0;
+        for (int i = tid; i < kBuckets; i += kThreads) hcount[i] = 0;
         __syncthreads();
       }
+      u64 m = 0;
       int above = 0;
+      const bool sums = masses && level == 0;
+#pragma unroll 4
       for (int i = tid; i < len; i += kThreads) {
         const float z = value(i);
-        int b = bucket(z);
-        if (level) {
-          if (b != b0) continue;
-          b = within_bucket(z, b0);
-        }
-        atomicAdd(&hcount[b], 1);
-        if (masses || (first && min_p > 0.f)) {
+        const int b = bucket(z, level, b0);
+        if (b >= 0) atomicAdd(&hcount[b], 1);
+        if (sums) {
           const double w = weight(r, z);
-          if (masses) {
-            const u64 m = to_mass(r, w);
-            if (m) atomicAdd(&hmass[b], m);
-          }
+          m += to_mass(r, w);
           above += w >= (double)min_p;
         }
       }
-      if (first && min_p > 0.f) {
-        for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-        if (lane == 0) atomicAdd(&sh.count, above);
+      if (sums) {
+        m = block_sum(m, sh);
+        above = __reduce_add_sync(0xffffffffu, above);
+        if (tid == 0) sh.mass = m;
+        if (lane == 0 && first) atomicAdd(&sh.count, above);
       }
-    } else {  // kGather
+    } else if (cmd == kMass) {
+      if (tid < kWindow) sh.window[tid] = 0;
+      __syncthreads();
+      u64 m = 0;
+#pragma unroll 4
       for (int i = tid; i < len; i += kThreads) {
         const float z = value(i);
-        int b = bucket(z);
-        if (level) {
-          if (b != b0) continue;
-          b = within_bucket(z, b0);
+        const int b = bucket(z, level, b0) - glo;
+        if (b >= -glo && b < kWindow) {
+          const u64 x = to_mass(r, weight(r, z));
+          if (b < 0) m += x; else if (x) atomicAdd(&sh.window[b], x);
         }
-        if (b >= glo && b <= ghi) {
-          const int p = atomicAdd(&boss->listed, 1);
-          if (p < kList) boss_list[p] = (u64)ordered(z) << 32 | (0xffffffffu - (uint32_t)(lo + i));
+      }
+      m = block_sum(m, sh);
+      if (tid == 0) sh.mass = m;
+    } else {  // kGather
+      for (int i0 = 0; i0 < len; i0 += kThreads) {
+        const int i = i0 + tid;
+        const float z = i < len ? value(i) : -INFINITY;
+        const int b = i < len ? bucket(z, level, b0) : -1;
+        const bool in = b >= glo && b <= ghi;
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (who) {
+          int p = 0;
+          if (lane == 0) p = atomicAdd(&boss->listed, __popc(who));
+          p = __shfl_sync(0xffffffffu, p, 0) + __popc(who & ((1u << lane) - 1));
+          if (in && p < kList) boss_list[p] = (u64)ordered(z) << 32 | (0xffffffffu - (uint32_t)(lo + i));
         }
       }
     }
     cluster.sync();
     if (rank == 0) {
-      int next = -1, bc = -1;
+      int next = -1;
+      constexpr int kPer = kBuckets / kThreads;
+      // first bucket that fulfils a condition that, once met, stays met
+      auto find = [&](auto cond) {
+        int mine = kBuckets;
+#pragma unroll
+        for (int j = kPer - 1; j >= 0; --j)
+          if (cond(tid * kPer + j)) mine = tid * kPer + j;
+        return block_min(mine, sh);
+      };
+      auto before_bucket = [&](int b) { return b > 0 ? (u64)hcount[b - 1] : 0ull; };
+      // a window around the bucket where the guessed masses reach `want`
+      // beyond bucket `from`, whose mass in front is `have`
+      auto aim = [&](u64 want, int from, u64 have, int most) {
+        const double f = total ? (double)gtotal / (double)total : 1.0, g0 = from > 0 ? (double)guess[from - 1] : 0.0;
+        const double x = g0 + ((double)want - (double)have) * (level ? 1.0 : f);
+        const int b = min(find([&](int i) { return (double)guess[i] >= x; }), most);
+        glo = max(0, min(b, kBuckets - 1) - kWindow / 2);
+        next = kMass;
+      };
+      int bk = kBuckets;  // the bucket in which the count reaches k_eff
       if (cmd == kHist) {
-        // the cluster's histogram, then its running sums in place
-        constexpr int kPer = kBuckets / kThreads;
-        u64 c[kPer], m[kPer], cs = 0, ms = 0;
+        // the cluster's counts, running sums in place, and the guessed masses
+        int c[kPer] = {};
+        static_assert(kPer == 4, "");
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) c[j] = m[j] = 0;
-        for (int k = 0; k < C; ++k) {
-          const int *rc = cluster.map_shared_rank(hcount, k) + tid * kPer;
-          const u64 *rm = cluster.map_shared_rank(hmass, k) + tid * kPer;
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            c[j] += rc[j];
-            if (masses) m[j] += rm[j];
+        for (int k = 0; k < kMaxCluster; ++k)
+          if (k < C) {
+            const int4 x = reinterpret_cast<const int4 *>(cluster.map_shared_rank(hcount, k))[tid];
+            c[0] += x.x, c[1] += x.y, c[2] += x.z, c[3] += x.w;
           }
-        }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) cs += c[j], ms += m[j];
-        u64 cb = block_before(cs, sh), mb = masses ? block_before(ms, sh) : 0;
-        // hcount / hmass: sums up to and with a bucket, within this level
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          cb += c[j], mb += m[j];
-          hcount[tid * kPer + j] = (int)cb;
-          hmass[tid * kPer + j] = mb;
-        }
-        __syncthreads();
-        if (level == 0) {
-          total = hmass[kBuckets - 1];
-          cbase = mbase = 0;
+        if (level == 0 && masses) {
+          total = 0;
+          for (int k = 0; k < C; ++k) total += cluster.map_shared_rank(&sh, k)->mass;
         }
         if (first) {
           k_eff = top_k > 0 ? min(top_k, n) : n;
@@ -449,138 +498,213 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
             k_eff = min(k_eff, max(k, 1ull));
           }
         }
-        if (top_p < 1.f && !p_mass) p_mass = max((u64)ceil(fmax((double)top_p, 0.0) * (double)total), 1ull);
-      }
-      const bool had_hist = cmd == kHist;
-      if (had_hist) {
-        // ---- the bucket in which the count reaches k_eff, or the mass p_mass
-        // (the cut), or in which the mass passes the draw's target
-        int mine = kBuckets;
-        for (int i = tid; i < kBuckets; i += kThreads) {
-          const u64 cc = cbase + (u64)hcount[i], mm = mbase + hmass[i];
-          const bool hit = drawing ? mm > target : cc >= k_eff || (p_mass && mm >= p_mass);
-          if (hit) {
-            mine = i;
-            break;
-          }
+        if (top_p < 1.f) p_mass = max((u64)ceil(fmax((double)top_p, 0.0) * (double)total), 1ull);
+        u64 g[kPer], cs = 0, gs = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          // level 1: parts of one bucket weigh the same
+          const float mid = level ? (float)b0 + 0.5f : (float)(tid * kPer + j) + 0.5f;
+          const float w = exp2f(-mid * ((float)(r.s + 2) / (float)(kBuckets - 1)));
+          g[j] = (u64)((double)c[j] * (double)w * r.unit);
+          cs += (u64)c[j];
+          gs += g[j];
         }
-        for (int o = 16; o > 0; o >>= 1) mine = min(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        u64 cb = block_before(cs, sh), gb = block_before(gs, sh);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          cb += (u64)c[j], gb += g[j];
+          hcount[tid * kPer + j] = (int)cb;
+          guess[tid * kPer + j] = gb;
+        }
         __syncthreads();
-        if (lane == 0) sh.red[warp] = mine;
-        __syncthreads();
-        bc = kBuckets;
-        for (int i = 0; i < kThreads / 32; ++i) bc = min(bc, (int)sh.red[i]);
-        if (!drawing && level == 0 && bc >= kBuckets - 1) {
-          // no cut among the tokens that count
-          if (!masses) {
+        gtotal = guess[kBuckets - 1];
+        if (level == 0) cup = mup = 0;
+        tries = 0;
+      }
+      if (cmd != kGather && !drawing) {
+        bk = find([&](int i) { return cup + (u64)hcount[i] >= k_eff; });
+        if (level == 0 && bk == kBuckets - 1) bk = kBuckets;  // cuts off nothing that counts
+      }
+      if (cmd == kHist) {
+        if (drawing) {
+          aim(target + 1, 0, mup, kBuckets - 1);
+        } else if (level == 0 && bk == kBuckets && !p_mass) {
+          if (!masses) {  // fewer tokens than top_k: all masses are needed after all
             masses = true;
             next = kHist;
           } else {
             kept = total;
             target = min((u64)(u * (double)kept), kept - 1);
             drawing = true;
-            mine = kBuckets;
-            for (int i = tid; i < kBuckets; i += kThreads)
-              if (hmass[i] > target) {
-                mine = i;
-                break;
-              }
-            for (int o = 16; o > 0; o >>= 1) mine = min(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-            __syncthreads();
-            if (lane == 0) sh.red[warp] = mine;
-            __syncthreads();
-            bc = kBuckets;
-            for (int i = 0; i < kThreads / 32; ++i) bc = min(bc, (int)sh.red[i]);
+            aim(target + 1, 0, 0, kBuckets - 1);
           }
-        }
-        if (next < 0) {
-          bc = min(bc, kBuckets - 1);
-          const int upto = hcount[bc], alone = upto - (bc ? hcount[bc - 1] : 0);
-          if (!drawing && level == 0 && upto <= kList) {
+        } else {
+          // when few: all of them, up to the cut (for top-p a little beyond its guess)
+          int upto = bk;
+          if (level == 0 && p_mass) {
+            const double x = (double)p_mass * 1.03 * ((double)gtotal / (double)total);
+            upto = min(upto, find([&](int i) { return (double)guess[i] >= x; }));
+          }
+          upto = min(upto, kBuckets - 2);
+          if (level == 0 && hcount[upto] <= kList) {
             next = kGather;
             glo = 0;
-            ghi = bc;
+            ghi = upto;
             cbase = mbase = 0;
+            whole_list = true;
           } else if (!masses) {
-            masses = true;  // what lies before the bucket is needed
+            masses = true;  // what lies before the cut's bucket is needed
             next = kHist;
-          } else if (alone <= kList || level == 0) {
-            if (bc) cbase += (u64)hcount[bc - 1], mbase += hmass[bc - 1];
-            if (alone <= kList) {
-              next = kGather;
-              glo = ghi = bc;
-            } else {
-              next = kHist;
-              level = 1;
-              b0 = bc;
-            }
+          } else if (p_mass) {
+            aim(p_mass, 0, mup, bk);
           } else {
-            const int token = long_way(r, zrow, n, k_eff, p_mass, u, hmass, sh, &kept);
-            if (tid == 0) finish(min(max(token, 0), n - 1), kept);
-            next = kDone;
+            glo = max(0, bk - kWindow / 2);
+            next = kMass;
+          }
+        }
+      } else if (cmd == kMass) {
+        // ---- exact masses around the guess
+        u64 e = mup, mine = 0;
+        for (int k = 0; k < C; ++k) {
+          e += cluster.map_shared_rank(&sh, k)->mass;
+          if (tid < kWindow) mine += cluster.map_shared_rank(&sh, k)->window[tid];
+        }
+        const u64 front = e + block_before(mine, sh), back = front + mine;
+        const u64 want = drawing ? target + 1 : p_mass;
+        int hit = kBuckets;
+        if (tid < kWindow && glo + tid < kBuckets && want && back >= want) hit = glo + tid;
+        hit = block_min(hit, sh);
+        const int end = min(kBuckets, glo + kWindow);
+        int b = kBuckets;
+        if (want && e >= want) {
+          b = -1;  // before the window
+        } else {
+          b = min(hit, drawing ? kBuckets : bk);
+          if (b >= end) b = kBuckets;  // behind it
+        }
+        if (b >= 0 && b < kBuckets) {
+          __syncthreads();
+          if (tid == b - glo) sh.pick = front;
+          __syncthreads();
+          const u64 alone = (u64)hcount[b] - before_bucket(b);
+          cbase = cup + before_bucket(b);
+          mbase = sh.pick;
+          if (alone <= kList) {
+            next = kGather;
+            glo = ghi = b;
+            whole_list = false;
+          } else if (level == 0) {
+            next = kHist;
+            level = 1;
+            b0 = b;
+            cup = cbase, mup = mbase;
+          }
+        } else if (++tries < 32) {
+          // aim again from this window's exact edge
+          __syncthreads();
+          if (tid == kWindow - 1) sh.pick = back;
+          __syncthreads();
+          const u64 edge = sh.pick;
+          const int was = glo;
+          if (b < 0) {
+            aim(want, was, e, kBuckets - 1);
+            glo = max(0, min(glo, was - kWindow));
+          } else {
+            aim(want ? want : edge, end, edge, drawing ? kBuckets - 1 : bk);
+            glo = max(glo, min(end, kBuckets - 1));
           }
         }
       } else {
         // ---- sort what was gathered (falling value, rising index), running masses
         const int cnt = min(sh.listed, kList);
-        int size = 2;
-        while (size < cnt) size <<= 1;
-        for (int i = cnt + tid; i < size; i += kThreads) list[i] = 0;
-        __syncthreads();
-        for (int k = 2; k <= size; k <<= 1)
-          for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int e = tid; e < size / 2; e += kThreads) {
-              const int x = 2 * e - (e & (j - 1)), y = x + j;
-              const u64 p = list[x], q = list[y];
-              if ((p < q) == ((x & k) == 0)) list[x] = q, list[y] = p;
+        u64 *sorted = list;
+        if (cnt <= kThreads) {
+          // each thread counts the elements before its own
+          sorted = list + kList / 2;
+          const u64 x = tid < cnt ? list[tid] : 0;
+          int place = 0;
+#pragma unroll 8
+          for (int i = 0; i < cnt; ++i) place += list[i] > x;
+          if (tid < cnt) sorted[place] = x;
+          __syncthreads();
+        } else {
+          int size = 2 * kThreads;
+          while (size < cnt) size <<= 1;
+          for (int i = cnt + tid; i < size; i += kThreads) list[i] = 0;
+          __syncthreads();
+          for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+              for (int e = tid; e < size / 2; e += kThreads) {
+                const int x = 2 * e - (e & (j - 1)), y = x + j;
+                const u64 p = list[x], q = list[y];
+                if ((p < q) == ((x & k) == 0)) list[x] = q, list[y] = p;
+              }
+              __syncthreads();
             }
-            __syncthreads();
-          }
-        constexpr int kPer = kList / kThreads;
-        u64 m[kPer], ms = 0;
+        }
+        const int each = cnt <= kThreads ? 1 : kList / kThreads;
+        u64 m[kList / kThreads], ms = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int i = tid * kPer + j;
-          m[j] = i < cnt ? to_mass(r, weight(r, unordered((uint32_t)(list[i] >> 32)))) : 0;
+        for (int j = 0; j < kList / kThreads; ++j) {
+          const int i = tid * each + j;
+          m[j] = j < each && i < cnt ? to_mass(r, weight(r, unordered((uint32_t)(sorted[i] >> 32)))) : 0;
           ms += m[j];
         }
         const u64 before = mbase + block_before(ms, sh);
+        bool cut = true;
         if (!drawing) {
           // how many are kept, and their mass
-          u64 keep = k_eff - min(k_eff, cbase), run = before;
-          if (tid == 0) sh.pick = min(keep, (u64)cnt);
+          const u64 room = k_eff - min(k_eff, cbase);
+          u64 keep = min(room, (u64)cnt), run = before;
+          if (tid == 0) sh.pick = kList + 1;
           __syncthreads();
           if (p_mass) {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-              if (run < p_mass && run + m[j] >= p_mass) atomicMin(&sh.pick, (u64)(tid * kPer + j + 1));
+            for (int j = 0; j < kList / kThreads; ++j) {
+              if (run < p_mass && run + m[j] >= p_mass) sh.pick = (u64)(tid * each + j + 1);
               run += m[j];
             }
           }
           __syncthreads();
-          keep = sh.pick;
+          const u64 by_mass = sh.pick;
+          cut = !whole_list || by_mass <= kList || room <= (u64)cnt;
+          keep = min(keep, by_mass);
           u64 inside = 0;
 #pragma unroll
-          for (int j = 0; j < kPer; ++j)
-            if ((u64)(tid * kPer + j) < keep) inside += m[j];
+          for (int j = 0; j < kList / kThreads; ++j)
+            if ((u64)(tid * each + j) < keep) inside += m[j];
           kept = mbase + block_sum(inside, sh);
           target = min((u64)(u * (double)kept), kept - 1);
-          drawing = true;
         }
-        if (target >= mbase) {
-          u64 run = before;
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            if (run <= target && target < run + m[j])
-              finish((int)(0xffffffffu - (uint32_t)list[tid * kPer + j]), kept);
-            run += m[j];
-          }
-          next = kDone;
+        if (!cut) {
+          // the mass was not reached: where it is needs exact sums
+          bk = find([&](int i) { return cup + (u64)hcount[i] >= k_eff; });
+          aim(p_mass, 0, 0, bk);
         } else {
-          // the draw falls before the cut's bucket: find its own
-          next = kHist;
-          level = 0;
+          drawing = true;
+          if (target >= mbase) {
+            u64 run = before;
+#pragma unroll
+            for (int j = 0; j < kList / kThreads; ++j) {
+              if (run <= target && target < run + m[j])
+                finish((int)(0xffffffffu - (uint32_t)sorted[tid * each + j]), kept);
+              run += m[j];
+            }
+            next = kDone;
+          } else if (level == 0) {
+            tries = 0;
+            mup = cup = 0;
+            aim(target + 1, 0, 0, kBuckets - 1);
+          } else {
+            next = kHist;  // the draw falls before the bucket that was split
+            level = 0;
+          }
         }
+      }
+      if (next < 0) {
+        const int token = long_way(r, zrow, n, k_eff, p_mass, u, guess, sh, &kept);
+        if (tid == 0) finish(min(max(token, 0), n - 1), kept);
+        next = kDone;
       }
       __syncthreads();
       if (tid == 0) {
@@ -589,20 +713,20 @@ __global__ void __launch_bounds__(kThreads) sample_rows_kernel(const __grid_cons
         sh.b0 = b0;
         sh.lo = glo;
         sh.hi = ghi;
+        sh.masses = masses;
         sh.listed = 0;
-        sh.count = masses;
       }
     }
     cluster.sync();
+    // read before the next barrier, behind which the leader gives new orders
     cmd = boss->cmd;
     level = boss->level;
     b0 = boss->b0;
     glo = boss->lo;
     ghi = boss->hi;
-    masses = boss->count;
+    masses = boss->masses;
     first = false;
     if (cmd == kDone) break;
-    cluster.sync();  // the orders are read before the leader gives new ones
   }
   cluster.sync();  // the leader's orders are read before it leaves
 }
