@@ -10,7 +10,7 @@
 // passes a target. Tokens are counted in 2048 buckets of equal width in z
 // (the last one takes all whose weight rounds to 0). A bucket is so narrow
 // that its count times the weight of its middle is its mass to 1%: that
-// guesses the place, and one pass that sums the masses before a window of 64
+// guesses the place, and one pass that sums the masses before a window of 16
 // buckets and of each bucket in it makes it exact. The bucket (or, when they
 // are few, all up to it) is gathered and sorted.
 //
@@ -36,7 +36,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512;
 constexpr int kBuckets = 2048;
 constexpr int kList = 2048;      // elements a gather can hold
-constexpr int kWindow = 64;      // buckets whose masses one pass makes exact
+constexpr int kWindow = 16;      // buckets whose masses one pass makes exact
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunk = 36864; // elements of a row that one CTA keeps in shared memory
 
@@ -88,18 +88,43 @@ __device__ __forceinline__ u64 to_mass(const Row &r, double w) {
 }
 
 // ------------------------------------------------ block-wide sums and scans
+// What the leader CTA knows, kept in shared memory between its turns.
+struct Book {
+  u64 total = 0, gtotal = 0;   // the row's mass, exact and guessed
+  u64 k_eff = 0, p_mass = 0;   // the count and the mass that are kept (0: no top-p)
+  u64 kept = 0, target = 0;    // kept mass, and the draw's place in it
+  u64 cbase = 0, mbase = 0;    // count and mass before what is gathered
+  u64 cup = 0, mup = 0;        // ... before the bucket that level 1 splits
+  int drawing = 0, whole_list = 0, tries = 0;
+};
+
+// One row's task: the logits, the settings, where the answer goes.
+struct Task {
+  Row row;
+  const float *z;
+  int *token;
+  float *logprob;
+  double u, inv_t;
+  float top_p, min_p;
+  int n, top_k;
+};
+
 struct Shared {
+  Task task;
+  Book book;
   double pow2[32];
   u64 red[kThreads / 32];
   u64 best;            // this CTA's largest value and its last index
   u64 mass;            // this CTA's mass: of all its tokens, or before the window
   u64 window[kWindow]; // ... and of each bucket in it
+  u64 parts[kThreads / 32][kWindow];  // the same by warp
   u64 pick;
   int count, listed;   // tokens with w >= min_p; length of the list
+  int place;
   float zmax;
   int last;
   // the leader's orders to the cluster
-  int cmd, level, b0, lo, hi, masses;
+  int cmd, level, b0, lo, hi, masses, first;
 };
 enum { kDone, kHist, kMass, kGather };
 
@@ -225,12 +250,306 @@ __device__ int long_way(const Row &r, const float *z, int n, u64 k_eff, u64 p_ma
   return c.idx;
 }
 
+// ------------------------------------------------------- the leader's turn
+// Between two passes of the cluster the leader CTA reads what the pass found
+// and gives the next orders. A function of its own, so that its registers
+// are not held during the passes.
+__device__ __forceinline__ void finish(const Task &t, int token, u64 kept) {  // one thread
+  *t.token = token;
+  if (t.logprob) {
+    const float z = clean(t.z[token]);
+    const double x = z == t.row.zmax ? 0.0 : ((double)z - (double)t.row.zmax) * t.inv_t;
+    *t.logprob = (float)(x - log((double)kept / t.row.unit));
+  }
+}
+
+__device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int *hcount) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), tid = threadIdx.x;
+  const Task &t = sh.task;
+  const Row &r = t.row;
+  const int n = t.n, cmd = sh.cmd;
+  int level = sh.level, b0 = sh.b0, glo = sh.lo, ghi = sh.hi;
+  bool masses = sh.masses;
+  const bool first = sh.first;
+  Book k = sh.book;
+  int next = -1;
+  constexpr int kPer = kBuckets / kThreads;
+  // first bucket that fulfils a condition that, once met, stays met
+  auto find = [&](auto cond) {
+    int mine = kBuckets;
+#pragma unroll
+    for (int j = kPer - 1; j >= 0; --j)
+      if (cond(tid * kPer + j)) mine = tid * kPer + j;
+    return block_min(mine, sh);
+  };
+  auto before_bucket = [&](int b) { return b > 0 ? (u64)hcount[b - 1] : 0ull; };
+  // a window around the bucket where the guessed masses reach `want`
+  // beyond bucket `from`, whose mass in front is `have`
+  auto aim = [&](u64 want, int from, u64 have, int most) {
+    const double f = k.total ? (double)k.gtotal / (double)k.total : 1.0, g0 = from > 0 ? (double)guess[from - 1] : 0.0;
+    const double x = g0 + ((double)want - (double)have) * (level ? 1.0 : f);
+    const int b = min(find([&](int i) { return (double)guess[i] >= x; }), most);
+    glo = max(0, min(b, kBuckets - 1) - kWindow / 2);
+    next = kMass;
+  };
+  int bk = kBuckets;  // the bucket in which the count reaches k.k_eff
+  if (cmd == kHist) {
+    // the cluster's counts, running sums in place, and the guessed masses
+    int c[kPer] = {};
+    static_assert(kPer == 4, "");
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q)
+      if (q < C) {
+        const int4 x = reinterpret_cast<const int4 *>(cluster.map_shared_rank(hcount, q))[tid];
+        c[0] += x.x, c[1] += x.y, c[2] += x.z, c[3] += x.w;
+      }
+    if (level == 0 && masses) {
+      k.total = 0;
+      for (int q = 0; q < C; ++q) k.total += cluster.map_shared_rank(&sh, q)->mass;
+    }
+    if (first) {
+      k.k_eff = t.top_k > 0 ? min(t.top_k, n) : n;
+      if (t.min_p > 0.f) {
+        u64 above = 0;
+        for (int q = 0; q < C; ++q) above += cluster.map_shared_rank(&sh, q)->count;
+        k.k_eff = min(k.k_eff, max(above, 1ull));
+      }
+    }
+    if (t.top_p < 1.f) k.p_mass = max((u64)ceil(fmax((double)t.top_p, 0.0) * (double)k.total), 1ull);
+    u64 g[kPer], cs = 0, gs = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      // level 1: parts of one bucket weigh the same
+      const float mid = level ? (float)b0 + 0.5f : (float)(tid * kPer + j) + 0.5f;
+      const float w = exp2f(-mid * ((float)(r.s + 2) / (float)(kBuckets - 1)));
+      g[j] = (u64)((double)c[j] * (double)w * r.unit);
+      cs += (u64)c[j];
+      gs += g[j];
+    }
+    u64 cb = block_before(cs, sh), gb = block_before(gs, sh);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      cb += (u64)c[j], gb += g[j];
+      hcount[tid * kPer + j] = (int)cb;
+      guess[tid * kPer + j] = gb;
+    }
+    __syncthreads();
+    k.gtotal = guess[kBuckets - 1];
+    if (level == 0) k.cup = k.mup = 0;
+    k.tries = 0;
+  }
+  if (cmd != kGather && !k.drawing) {
+    bk = find([&](int i) { return k.cup + (u64)hcount[i] >= k.k_eff; });
+    if (level == 0 && bk == kBuckets - 1) bk = kBuckets;  // cuts off nothing that counts
+  }
+  if (cmd == kHist) {
+    if (k.drawing) {
+      aim(k.target + 1, 0, k.mup, kBuckets - 1);
+    } else if (level == 0 && bk == kBuckets && !k.p_mass) {
+      if (!masses) {  // fewer tokens than top_k: all masses are needed after all
+        masses = true;
+        next = kHist;
+      } else {
+        k.kept = k.total;
+        k.target = min((u64)(t.u * (double)k.kept), k.kept - 1);
+        k.drawing = true;
+        aim(k.target + 1, 0, 0, kBuckets - 1);
+      }
+    } else {
+      // when few: all of them, up to the cut (for top-p a little beyond its guess)
+      int upto = bk;
+      if (level == 0 && k.p_mass) {
+        const double x = (double)k.p_mass * 1.03 * ((double)k.gtotal / (double)k.total);
+        upto = min(upto, find([&](int i) { return (double)guess[i] >= x; }));
+      }
+      upto = min(upto, kBuckets - 2);
+      if (level == 0 && hcount[upto] <= kList) {
+        next = kGather;
+        glo = 0;
+        ghi = upto;
+        k.cbase = k.mbase = 0;
+        k.whole_list = true;
+      } else if (!masses) {
+        masses = true;  // what lies before the cut's bucket is needed
+        next = kHist;
+      } else if (k.p_mass) {
+        aim(k.p_mass, 0, k.mup, bk);
+      } else {
+        glo = max(0, bk - kWindow / 2);
+        next = kMass;
+      }
+    }
+  } else if (cmd == kMass) {
+    // ---- exact masses around the guess
+    u64 e = k.mup, mine = 0;
+    for (int q = 0; q < C; ++q) {
+      e += cluster.map_shared_rank(&sh, q)->mass;
+      if (tid < kWindow) mine += cluster.map_shared_rank(&sh, q)->window[tid];
+    }
+    const u64 front = e + block_before(mine, sh), back = front + mine;
+    const u64 want = k.drawing ? k.target + 1 : k.p_mass;
+    int hit = kBuckets;
+    if (tid < kWindow && glo + tid < kBuckets && want && back >= want) hit = glo + tid;
+    hit = block_min(hit, sh);
+    const int end = min(kBuckets, glo + kWindow);
+    int b = kBuckets;
+    if (want && e >= want) {
+      b = -1;  // before the window
+    } else {
+      b = min(hit, k.drawing ? kBuckets : bk);
+      if (b >= end) b = kBuckets;  // behind it
+    }
+    if (b >= 0 && b < kBuckets) {
+      __syncthreads();
+      if (tid == b - glo) sh.pick = front;
+      __syncthreads();
+      const u64 alone = (u64)hcount[b] - before_bucket(b);
+      k.cbase = k.cup + before_bucket(b);
+      k.mbase = sh.pick;
+      if (alone <= kList) {
+        next = kGather;
+        glo = ghi = b;
+        k.whole_list = false;
+      } else if (level == 0) {
+        next = kHist;
+        level = 1;
+        b0 = b;
+        k.cup = k.cbase, k.mup = k.mbase;
+      }
+    } else if (++k.tries < 32) {
+      // aim again from this window's exact edge
+      __syncthreads();
+      if (tid == kWindow - 1) sh.pick = back;
+      __syncthreads();
+      const u64 edge = sh.pick;
+      const int was = glo;
+      if (b < 0) {
+        aim(want, was, e, kBuckets - 1);
+        glo = max(0, min(glo, was - kWindow));
+      } else {
+        aim(want ? want : edge, end, edge, k.drawing ? kBuckets - 1 : bk);
+        glo = max(glo, min(end, kBuckets - 1));
+      }
+    }
+  } else {
+    // ---- sort what was gathered (falling value, rising index), running masses
+    const int cnt = min(sh.listed, kList);
+    u64 *sorted = list;
+    if (cnt <= kList / 2) {
+      // each thread counts the elements before its own (two at most), two a load
+      sorted = list + kList / 2;
+      if (tid == 0 && (cnt & 1)) list[cnt] = 0;
+      __syncthreads();
+      const u64 x = tid < cnt ? list[tid] : 0, y = tid + kThreads < cnt ? list[tid + kThreads] : 0;
+      int px = 0, py = 0;
+#pragma unroll 4
+      for (int i = 0; i < cnt; i += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(list + i);
+        px += (q.x > x) + (q.y > x);
+        py += (q.x > y) + (q.y > y);
+      }
+      if (tid < cnt) sorted[px] = x;
+      if (tid + kThreads < cnt) sorted[py] = y;
+      __syncthreads();
+    } else {
+      int size = 2 * kThreads;
+      while (size < cnt) size <<= 1;
+      for (int i = cnt + tid; i < size; i += kThreads) list[i] = 0;
+      __syncthreads();
+      for (int half = 2; half <= size; half <<= 1)
+        for (int j = half >> 1; j > 0; j >>= 1) {
+          for (int e = tid; e < size / 2; e += kThreads) {
+            const int x = 2 * e - (e & (j - 1)), y = x + j;
+            const u64 p = list[x], q = list[y];
+            if ((p < q) == ((x & half) == 0)) list[x] = q, list[y] = p;
+          }
+          __syncthreads();
+        }
+    }
+    const int each = cnt <= kThreads ? 1 : cnt <= kList / 2 ? 2 : kList / kThreads;
+    u64 m[kList / kThreads], ms = 0;
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j) {
+      const int i = tid * each + j;
+      m[j] = j < each && i < cnt ? to_mass(r, weight(r, unordered((uint32_t)(sorted[i] >> 32)))) : 0;
+      ms += m[j];
+    }
+    const u64 before = k.mbase + block_before(ms, sh);
+    bool cut = true;
+    if (!k.drawing) {
+      // how many are k.kept, and their mass
+      const u64 room = k.k_eff - min(k.k_eff, k.cbase);
+      u64 keep = min(room, (u64)cnt), run = before;
+      if (tid == 0) sh.pick = kList + 1;
+      __syncthreads();
+      if (k.p_mass) {
+#pragma unroll
+        for (int j = 0; j < kList / kThreads; ++j) {
+          if (run < k.p_mass && run + m[j] >= k.p_mass) sh.pick = (u64)(tid * each + j + 1);
+          run += m[j];
+        }
+      }
+      __syncthreads();
+      const u64 by_mass = sh.pick;
+      cut = !k.whole_list || by_mass <= kList || room <= (u64)cnt;
+      keep = min(keep, by_mass);
+      u64 inside = 0;
+#pragma unroll
+      for (int j = 0; j < kList / kThreads; ++j)
+        if ((u64)(tid * each + j) < keep) inside += m[j];
+      k.kept = k.mbase + block_sum(inside, sh);
+      k.target = min((u64)(t.u * (double)k.kept), k.kept - 1);
+    }
+    if (!cut) {
+      // the mass was not reached: where it is needs exact sums
+      bk = find([&](int i) { return k.cup + (u64)hcount[i] >= k.k_eff; });
+      aim(k.p_mass, 0, 0, bk);
+    } else {
+      k.drawing = true;
+      if (k.target >= k.mbase) {
+        u64 run = before;
+#pragma unroll
+        for (int j = 0; j < kList / kThreads; ++j) {
+          if (run <= k.target && k.target < run + m[j])
+            finish(t, (int)(0xffffffffu - (uint32_t)sorted[tid * each + j]), k.kept);
+          run += m[j];
+        }
+        next = kDone;
+      } else if (level == 0) {
+        k.tries = 0;
+        k.mup = k.cup = 0;
+        aim(k.target + 1, 0, 0, kBuckets - 1);
+      } else {
+        next = kHist;  // the draw falls before the bucket that was split
+        level = 0;
+      }
+    }
+  }
+  if (next < 0) {
+    const int token = long_way(r, t.z, n, k.k_eff, k.p_mass, t.u, guess, sh, &k.kept);
+    if (tid == 0) finish(t, min(max(token, 0), n - 1), k.kept);
+    next = kDone;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    sh.book = k;
+    sh.cmd = next;
+    sh.level = level;
+    sh.b0 = b0;
+    sh.lo = glo;
+    sh.hi = ghi;
+    sh.masses = masses;
+    sh.listed = 0;
+  }
+}
+
 // --------------------------------------------------------------- the kernel
 // A cluster of gridDim.x CTAs per row. IN_SMEM: each CTA's share of the row
 // stays in its shared memory; otherwise every pass reads it from global
 // memory (rows beyond 8 * kMaxChunk tokens).
-template <bool IN_SMEM>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a) {
+template <bool IN_SMEM, int PER_SM>
+__global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a) {
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -244,6 +563,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   float *zs = reinterpret_cast<float *>(hcount + kBuckets);       // [per]
   auto value = [&](int i) { return IN_SMEM ? zs[i] : clean(zrow[lo + i]); };
 
+  const float T = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f;
+  const float min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f, u_row = a.u[row];
+  const int top_k = a.top_k ? a.top_k[row] : 0;
   if (tid < 32) sh.pow2[tid] = kPow2[tid];
   // ---- read the row; its largest value and the last index that has it
   float top = -INFINITY;
@@ -298,7 +620,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     }
   }
   __syncthreads();
-  const float T = a.temperature ? a.temperature[row] : 1.f;
   Row r;
   r.zmax = sh.zmax;
   const int last = sh.last;
@@ -318,18 +639,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   // below 2^-(s+2) of the maximum nothing counts
   r.cut = (r.s + 2) * 0.6931471805599453 * (double)T;
   const float scale = (float)(kBuckets - 1) / (float)r.cut;
-  const int top_k = a.top_k ? a.top_k[row] : 0;
-  const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
-  const double u = fmin(fmax((double)a.u[row], 0.0), 1.0);
-  auto finish = [&](int token, u64 kept) {  // one thread of the leader
-    a.token[row] = token;
-    if (a.logprob) {
-      const float z = clean(zrow[token]);
-      const double t = z == r.zmax ? 0.0 : ((double)z - (double)r.zmax) * fmax(1.0 / (double)T, 1e-300);
-      a.logprob[row] = (float)(t - log((double)kept / r.unit));
-    }
-  };
-
+  const double u = fmin(fmax((double)u_row, 0.0), 1.0);
+  if (tid == 0)
+    sh.task = Task{r,     zrow,  a.token + row, a.logprob ? a.logprob + row : nullptr, u, fmax(1.0 / (double)T, 1e-300),
+                   top_p, min_p, n,             top_k};
   if (top_k <= 0 && !(top_p < 1.f) && !(min_p > 0.f)) {
     // ---- no filter: the draw is in index order. Every warp sums a run of
     // its CTA's share; the one that holds the target walks its run again
@@ -367,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         for (int i = e0; i < e1; ++i) {
           before += to_mass(r, weight(r, value(i)));
           if (before > target) {
-            finish(lo + i, total);
+            finish(sh.task, lo + i, total);
             break;
           }
         }
@@ -388,15 +701,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
     if (level == 0) return b;
     return b == b0 ? min(kBuckets - 1, max(0, (int)(fmaf(d, scale, -(float)b0) * kBuckets))) : -1;
   };
+  // f(index of the first, values, whether there is one) for every kBatch
+  // tokens of a thread: loaded together, ahead of what f writes
+  constexpr int kBatch = PER_SM == 1 ? 4 : 2;
+  auto batches = [&](auto f) {
+    for (int i0 = 0; i0 < len; i0 += kBatch * kThreads) {
+      float z[kBatch];
+      bool in[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kThreads + tid;
+        in[j] = i < len;
+        z[j] = in[j] ? value(i) : -INFINITY;
+      }
+      f(i0 + tid, z, in);
+    }
+  };
   int cmd = kHist, level = 0, b0 = 0, glo = 0, ghi = 0;
   bool masses = top_p < 1.f || top_k <= 0 || top_k > kList / 2 || min_p > 0.f;  // the first pass sums them all
   bool first = true;
-  // the leader's bookkeeping, the same in all its threads
-  u64 total = 0, gtotal = 0, k_eff = 0, p_mass = 0, kept = 0, target = 0;
-  u64 cbase = 0, mbase = 0;  // count and mass before what is gathered
-  u64 cup = 0, mup = 0;      // ... before the bucket that level 1 splits
-  bool drawing = false, whole_list = false;
-  int tries = 0;
+  if (tid == 0) {
+    sh.book = Book{};
+    sh.cmd = cmd, sh.level = 0, sh.b0 = 0, sh.lo = sh.hi = 0, sh.masses = masses, sh.first = 1;
+  }
   for (;;) {
     if (cmd == kHist) {
       if (!first) {
@@ -406,17 +733,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
       u64 m = 0;
       int above = 0;
       const bool sums = masses && level == 0;
-#pragma unroll 4
-      for (int i = tid; i < len; i += kThreads) {
-        const float z = value(i);
-        const int b = bucket(z, level, b0);
-        if (b >= 0) atomicAdd(&hcount[b], 1);
-        if (sums) {
-          const double w = weight(r, z);
-          m += to_mass(r, w);
-          above += w >= (double)min_p;
+      batches([&](int, const float (&z)[kBatch], const bool (&in)[kBatch]) {
+        int b[kBatch];
+        double w[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          b[j] = in[j] ? bucket(z[j], level, b0) : -1;
+          if (sums) w[j] = weight(r, z[j]);  // of -inf where there is no token: 0
         }
-      }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          if (sums) {
+            m += to_mass(r, w[j]);
+            above += w[j] >= (double)min_p;
+          }
+          if (b[j] >= 0) atomicAdd(&hcount[b[j]], 1);
+        }
+      });
       if (sums) {
         m = block_sum(m, sh);
         above = __reduce_add_sync(0xffffffffu, above);
@@ -424,299 +757,61 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
         if (lane == 0 && first) atomicAdd(&sh.count, above);
       }
     } else if (cmd == kMass) {
-      if (tid < kWindow) sh.window[tid] = 0;
-      __syncthreads();
+      if (lane < kWindow) sh.parts[warp][lane] = 0;
+      __syncwarp();
       u64 m = 0;
-#pragma unroll 4
-      for (int i = tid; i < len; i += kThreads) {
-        const float z = value(i);
-        const int b = bucket(z, level, b0) - glo;
-        if (b >= -glo && b < kWindow) {
-          const u64 x = to_mass(r, weight(r, z));
-          if (b < 0) m += x; else if (x) atomicAdd(&sh.window[b], x);
+      batches([&](int, const float (&z)[kBatch], const bool (&in)[kBatch]) {
+        int b[kBatch];
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          b[j] = in[j] ? bucket(z[j], level, b0) : -1;
+          b[j] = b[j] < 0 ? kWindow : b[j] - glo;
+          any |= b[j] < kWindow;
         }
-      }
+        if (__any_sync(0xffffffffu, any)) {
+          u64 x[kBatch];
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) x[j] = to_mass(r, weight(r, z[j]));
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j)
+            if (b[j] < 0) m += x[j]; else if (b[j] < kWindow && x[j]) atomicAdd(&sh.parts[warp][b[j]], x[j]);
+        }
+      });
       m = block_sum(m, sh);
       if (tid == 0) sh.mass = m;
-    } else {  // kGather
-      for (int i0 = 0; i0 < len; i0 += kThreads) {
-        const int i = i0 + tid;
-        const float z = i < len ? value(i) : -INFINITY;
-        const int b = i < len ? bucket(z, level, b0) : -1;
-        const bool in = b >= glo && b <= ghi;
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (who) {
-          int p = 0;
-          if (lane == 0) p = atomicAdd(&boss->listed, __popc(who));
-          p = __shfl_sync(0xffffffffu, p, 0) + __popc(who & ((1u << lane) - 1));
-          if (in && p < kList) boss_list[p] = (u64)ordered(z) << 32 | (0xffffffffu - (uint32_t)(lo + i));
-        }
+      if (tid < kWindow) {
+        u64 t = 0;
+        for (int i = 0; i < kThreads / 32; ++i) t += sh.parts[i][tid];
+        sh.window[tid] = t;
       }
+    } else {  // kGather: count, take places in the leader's list, write
+      int hits = 0;
+      batches([&](int, const float (&z)[kBatch], const bool (&in)[kBatch]) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int b = in[j] ? bucket(z[j], level, b0) : -1;
+          hits += b >= glo && b <= ghi;
+        }
+      });
+      int p = (int)block_before((u64)hits, sh);
+      if (tid == kThreads - 1) sh.place = p + hits ? atomicAdd(&boss->listed, p + hits) : 0;
+      __syncthreads();
+      p += sh.place;
+      if (__any_sync(0xffffffffu, hits))
+        batches([&](int i, const float (&z)[kBatch], const bool (&in)[kBatch]) {
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const int b = in[j] ? bucket(z[j], level, b0) : -1;
+            if (b >= glo && b <= ghi) {
+              if (p < kList) boss_list[p] = (u64)ordered(z[j]) << 32 | (0xffffffffu - (uint32_t)(lo + i + j * kThreads));
+              ++p;
+            }
+          }
+        });
     }
     cluster.sync();
-    if (rank == 0) {
-      int next = -1;
-      constexpr int kPer = kBuckets / kThreads;
-      // first bucket that fulfils a condition that, once met, stays met
-      auto find = [&](auto cond) {
-        int mine = kBuckets;
-#pragma unroll
-        for (int j = kPer - 1; j >= 0; --j)
-          if (cond(tid * kPer + j)) mine = tid * kPer + j;
-        return block_min(mine, sh);
-      };
-      auto before_bucket = [&](int b) { return b > 0 ? (u64)hcount[b - 1] : 0ull; };
-      // a window around the bucket where the guessed masses reach `want`
-      // beyond bucket `from`, whose mass in front is `have`
-      auto aim = [&](u64 want, int from, u64 have, int most) {
-        const double f = total ? (double)gtotal / (double)total : 1.0, g0 = from > 0 ? (double)guess[from - 1] : 0.0;
-        const double x = g0 + ((double)want - (double)have) * (level ? 1.0 : f);
-        const int b = min(find([&](int i) { return (double)guess[i] >= x; }), most);
-        glo = max(0, min(b, kBuckets - 1) - kWindow / 2);
-        next = kMass;
-      };
-      int bk = kBuckets;  // the bucket in which the count reaches k_eff
-      if (cmd == kHist) {
-        // the cluster's counts, running sums in place, and the guessed masses
-        int c[kPer] = {};
-        static_assert(kPer == 4, "");
-#pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k)
-          if (k < C) {
-            const int4 x = reinterpret_cast<const int4 *>(cluster.map_shared_rank(hcount, k))[tid];
-            c[0] += x.x, c[1] += x.y, c[2] += x.z, c[3] += x.w;
-          }
-        if (level == 0 && masses) {
-          total = 0;
-          for (int k = 0; k < C; ++k) total += cluster.map_shared_rank(&sh, k)->mass;
-        }
-        if (first) {
-          k_eff = top_k > 0 ? min(top_k, n) : n;
-          if (min_p > 0.f) {
-            u64 k = 0;
-            for (int i = 0; i < C; ++i) k += cluster.map_shared_rank(&sh, i)->count;
-            k_eff = min(k_eff, max(k, 1ull));
-          }
-        }
-        if (top_p < 1.f) p_mass = max((u64)ceil(fmax((double)top_p, 0.0) * (double)total), 1ull);
-        u64 g[kPer], cs = 0, gs = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          // level 1: parts of one bucket weigh the same
-          const float mid = level ? (float)b0 + 0.5f : (float)(tid * kPer + j) + 0.5f;
-          const float w = exp2f(-mid * ((float)(r.s + 2) / (float)(kBuckets - 1)));
-          g[j] = (u64)((double)c[j] * (double)w * r.unit);
-          cs += (u64)c[j];
-          gs += g[j];
-        }
-        u64 cb = block_before(cs, sh), gb = block_before(gs, sh);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          cb += (u64)c[j], gb += g[j];
-          hcount[tid * kPer + j] = (int)cb;
-          guess[tid * kPer + j] = gb;
-        }
-        __syncthreads();
-        gtotal = guess[kBuckets - 1];
-        if (level == 0) cup = mup = 0;
-        tries = 0;
-      }
-      if (cmd != kGather && !drawing) {
-        bk = find([&](int i) { return cup + (u64)hcount[i] >= k_eff; });
-        if (level == 0 && bk == kBuckets - 1) bk = kBuckets;  // cuts off nothing that counts
-      }
-      if (cmd == kHist) {
-        if (drawing) {
-          aim(target + 1, 0, mup, kBuckets - 1);
-        } else if (level == 0 && bk == kBuckets && !p_mass) {
-          if (!masses) {  // fewer tokens than top_k: all masses are needed after all
-            masses = true;
-            next = kHist;
-          } else {
-            kept = total;
-            target = min((u64)(u * (double)kept), kept - 1);
-            drawing = true;
-            aim(target + 1, 0, 0, kBuckets - 1);
-          }
-        } else {
-          // when few: all of them, up to the cut (for top-p a little beyond its guess)
-          int upto = bk;
-          if (level == 0 && p_mass) {
-            const double x = (double)p_mass * 1.03 * ((double)gtotal / (double)total);
-            upto = min(upto, find([&](int i) { return (double)guess[i] >= x; }));
-          }
-          upto = min(upto, kBuckets - 2);
-          if (level == 0 && hcount[upto] <= kList) {
-            next = kGather;
-            glo = 0;
-            ghi = upto;
-            cbase = mbase = 0;
-            whole_list = true;
-          } else if (!masses) {
-            masses = true;  // what lies before the cut's bucket is needed
-            next = kHist;
-          } else if (p_mass) {
-            aim(p_mass, 0, mup, bk);
-          } else {
-            glo = max(0, bk - kWindow / 2);
-            next = kMass;
-          }
-        }
-      } else if (cmd == kMass) {
-        // ---- exact masses around the guess
-        u64 e = mup, mine = 0;
-        for (int k = 0; k < C; ++k) {
-          e += cluster.map_shared_rank(&sh, k)->mass;
-          if (tid < kWindow) mine += cluster.map_shared_rank(&sh, k)->window[tid];
-        }
-        const u64 front = e + block_before(mine, sh), back = front + mine;
-        const u64 want = drawing ? target + 1 : p_mass;
-        int hit = kBuckets;
-        if (tid < kWindow && glo + tid < kBuckets && want && back >= want) hit = glo + tid;
-        hit = block_min(hit, sh);
-        const int end = min(kBuckets, glo + kWindow);
-        int b = kBuckets;
-        if (want && e >= want) {
-          b = -1;  // before the window
-        } else {
-          b = min(hit, drawing ? kBuckets : bk);
-          if (b >= end) b = kBuckets;  // behind it
-        }
-        if (b >= 0 && b < kBuckets) {
-          __syncthreads();
-          if (tid == b - glo) sh.pick = front;
-          __syncthreads();
-          const u64 alone = (u64)hcount[b] - before_bucket(b);
-          cbase = cup + before_bucket(b);
-          mbase = sh.pick;
-          if (alone <= kList) {
-            next = kGather;
-            glo = ghi = b;
-            whole_list = false;
-          } else if (level == 0) {
-            next = kHist;
-            level = 1;
-            b0 = b;
-            cup = cbase, mup = mbase;
-          }
-        } else if (++tries < 32) {
-          // aim again from this window's exact edge
-          __syncthreads();
-          if (tid == kWindow - 1) sh.pick = back;
-          __syncthreads();
-          const u64 edge = sh.pick;
-          const int was = glo;
-          if (b < 0) {
-            aim(want, was, e, kBuckets - 1);
-            glo = max(0, min(glo, was - kWindow));
-          } else {
-            aim(want ? want : edge, end, edge, drawing ? kBuckets - 1 : bk);
-            glo = max(glo, min(end, kBuckets - 1));
-          }
-        }
-      } else {
-        // ---- sort what was gathered (falling value, rising index), running masses
-        const int cnt = min(sh.listed, kList);
-        u64 *sorted = list;
-        if (cnt <= kThreads) {
-          // each thread counts the elements before its own
-          sorted = list + kList / 2;
-          const u64 x = tid < cnt ? list[tid] : 0;
-          int place = 0;
-#pragma unroll 8
-          for (int i = 0; i < cnt; ++i) place += list[i] > x;
-          if (tid < cnt) sorted[place] = x;
-          __syncthreads();
-        } else {
-          int size = 2 * kThreads;
-          while (size < cnt) size <<= 1;
-          for (int i = cnt + tid; i < size; i += kThreads) list[i] = 0;
-          __syncthreads();
-          for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-              for (int e = tid; e < size / 2; e += kThreads) {
-                const int x = 2 * e - (e & (j - 1)), y = x + j;
-                const u64 p = list[x], q = list[y];
-                if ((p < q) == ((x & k) == 0)) list[x] = q, list[y] = p;
-              }
-              __syncthreads();
-            }
-        }
-        const int each = cnt <= kThreads ? 1 : kList / kThreads;
-        u64 m[kList / kThreads], ms = 0;
-#pragma unroll
-        for (int j = 0; j < kList / kThreads; ++j) {
-          const int i = tid * each + j;
-          m[j] = j < each && i < cnt ? to_mass(r, weight(r, unordered((uint32_t)(sorted[i] >> 32)))) : 0;
-          ms += m[j];
-        }
-        const u64 before = mbase + block_before(ms, sh);
-        bool cut = true;
-        if (!drawing) {
-          // how many are kept, and their mass
-          const u64 room = k_eff - min(k_eff, cbase);
-          u64 keep = min(room, (u64)cnt), run = before;
-          if (tid == 0) sh.pick = kList + 1;
-          __syncthreads();
-          if (p_mass) {
-#pragma unroll
-            for (int j = 0; j < kList / kThreads; ++j) {
-              if (run < p_mass && run + m[j] >= p_mass) sh.pick = (u64)(tid * each + j + 1);
-              run += m[j];
-            }
-          }
-          __syncthreads();
-          const u64 by_mass = sh.pick;
-          cut = !whole_list || by_mass <= kList || room <= (u64)cnt;
-          keep = min(keep, by_mass);
-          u64 inside = 0;
-#pragma unroll
-          for (int j = 0; j < kList / kThreads; ++j)
-            if ((u64)(tid * each + j) < keep) inside += m[j];
-          kept = mbase + block_sum(inside, sh);
-          target = min((u64)(u * (double)kept), kept - 1);
-        }
-        if (!cut) {
-          // the mass was not reached: where it is needs exact sums
-          bk = find([&](int i) { return cup + (u64)hcount[i] >= k_eff; });
-          aim(p_mass, 0, 0, bk);
-        } else {
-          drawing = true;
-          if (target >= mbase) {
-            u64 run = before;
-#pragma unroll
-            for (int j = 0; j < kList / kThreads; ++j) {
-              if (run <= target && target < run + m[j])
-                finish((int)(0xffffffffu - (uint32_t)sorted[tid * each + j]), kept);
-              run += m[j];
-            }
-            next = kDone;
-          } else if (level == 0) {
-            tries = 0;
-            mup = cup = 0;
-            aim(target + 1, 0, 0, kBuckets - 1);
-          } else {
-            next = kHist;  // the draw falls before the bucket that was split
-            level = 0;
-          }
-        }
-      }
-      if (next < 0) {
-        const int token = long_way(r, zrow, n, k_eff, p_mass, u, guess, sh, &kept);
-        if (tid == 0) finish(min(max(token, 0), n - 1), kept);
-        next = kDone;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        sh.cmd = next;
-        sh.level = level;
-        sh.b0 = b0;
-        sh.lo = glo;
-        sh.hi = ghi;
-        sh.masses = masses;
-        sh.listed = 0;
-      }
-    }
+    if (rank == 0) leader_turn(sh, list, guess, hcount);
     cluster.sync();
     // read before the next barrier, behind which the leader gives new orders
     cmd = boss->cmd;
@@ -731,9 +826,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const __grid_c
   cluster.sync();  // the leader's orders are read before it leaves
 }
 
-template <bool IN_SMEM>
+template <bool IN_SMEM, int PER_SM>
 ifx_status run(const SampleRowsArgs &a, int cluster, size_t smem, cudaStream_t st) {
-  auto kernel = sample_rows_kernel<IN_SMEM>;
+  auto kernel = sample_rows_kernel<IN_SMEM, PER_SM>;
   if (smem > 48 * 1024) IFX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
@@ -771,8 +866,12 @@ ifx_status op_sample_rows(const SampleRowsArgs &a, cudaStream_t st) {
   while (cluster < kMaxCluster && a.n > (int64_t)cluster * 2048) cluster *= 2;
   const int64_t per = ((a.n + cluster - 1) / cluster + 3) & ~(int64_t)3;
   const size_t base = kBuckets * (sizeof(u64) + sizeof(int)) + kList * sizeof(u64);
-  if (per <= kMaxChunk) return run<true>(a, cluster, base + (size_t)per * sizeof(float), st);
-  return run<false>(a, cluster, base, st);
+  const size_t smem = per <= kMaxChunk ? base + (size_t)per * sizeof(float) : base;
+  // few rows: more registers for a CTA that has its SM to itself; many: two
+  // CTAs an SM, one of which computes while the other waits
+  if (a.rows * cluster <= kNumSMs)
+    return per <= kMaxChunk ? run<true, 1>(a, cluster, smem, st) : run<false, 1>(a, cluster, smem, st);
+  return per <= kMaxChunk ? run<true, 2>(a, cluster, smem, st) : run<false, 2>(a, cluster, smem, st);
 }
 
 }  // namespace ifx
