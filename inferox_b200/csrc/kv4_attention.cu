@@ -780,7 +780,8 @@ ifx_status run(const Kv4AttnArgs &a, cudaStream_t st) {
   using L = Smem<NB, NT, NW>;
   auto kernel = kv4_attn_kernel<NB, NT, NW, MINB>;
   const size_t smem = L::kBytes + ((size_t)a.n_seqs + 1) * sizeof(long long);
-  IFX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes + (kMaxAttnSeqs + 1) * 8));
+  static std::atomic<uint64_t> done{0};
+  IFX_TRY(raise_smem(kernel, L::kBytes + (kMaxAttnSeqs + 1) * 8, done));
   const int grid = kNumSMs * MINB;
   kernel<<<grid, NW * 32, smem, st>>>(a);
   IFX_CUDA(cudaGetLastError());

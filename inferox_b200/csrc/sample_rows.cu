@@ -829,7 +829,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
 template <bool IN_SMEM, int PER_SM>
 ifx_status run(const SampleRowsArgs &a, int cluster, size_t smem, cudaStream_t st) {
   auto kernel = sample_rows_kernel<IN_SMEM, PER_SM>;
-  if (smem > 48 * 1024) IFX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+  static std::atomic<uint64_t> done{0};
+  if (smem > 48 * 1024) IFX_TRY(raise_smem(kernel, 220 * 1024, done));
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;

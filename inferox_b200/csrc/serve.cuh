@@ -1,6 +1,8 @@
 // The operators of a paged serving step: page tables and slot maps, the
 // key/value cache in 4 bits with its attention, and row-wise sampling.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ifx {
@@ -36,6 +38,19 @@ struct Kv4Layout {
 
 inline bool kv4_head_dim_ok(size_t hd) { return hd >= 32 && hd <= 256 && hd % 32 == 0; }
 inline size_t kv4_page_bytes(size_t G, size_t hd) { return G * (size_t)Kv4Layout::head_bytes((int)(hd / 32)); }
+
+// Raises a kernel's shared-memory limit, once per device: `done` holds a bit
+// for each (the call costs a microsecond or two).
+template <typename K>
+ifx_status raise_smem(K kernel, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  IFX_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return IFX_OK;
+  IFX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return IFX_OK;
+}
 
 struct PagesExtendArgs {
   const int *lens, *add;

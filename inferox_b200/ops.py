@@ -7,6 +7,7 @@ Shape mismatches raise IfxError("Shape") where the reference panics.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import NamedTuple
 
 import numpy as np
@@ -162,26 +163,26 @@ _TYPES = {torch.float32: 0, torch.float16: 1}
 
 def _dev(*tensors) -> int:
     """The one CUDA device the tensors are on."""
-    d = tensors[0].device
+    d = tensors[0].get_device()
     for t in tensors:
-        if t.device != d or not t.is_cuda:
+        if t.get_device() != d or d < 0:
             raise IfxError(24, "expected CUDA tensors of one device")
-    return d.index
+    return d
 
 
 def _ints(what: str, *tensors):
     for t in tensors:
-        if t.dtype != torch.int32 or not t.is_contiguous():
+        if t.dtype is not torch.int32 or not t.is_contiguous():
             raise IfxError(24, f"{what}: expected contiguous int32 tensors")
 
 
 def _call(dev: int, what: str, fn, *args):
     """fn(*args, stream) on the current stream of device `dev`."""
-    if dev == torch.cuda.current_device():
-        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if dev == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if code:
         check(code, what)
 
@@ -213,16 +214,16 @@ def pages_extend(lens, add, table, free, n_free, max_tokens: int) -> PageStep:
     _need(table.dim() == 2 and table.shape[0] == n and add.numel() == n and n_free.numel() == 1,
           "pages_extend shape mismatch")
     _need(max_tokens >= 0, "pages_extend: negative max_tokens")
-    # one allocation, its parts 16-byte aligned
-    m4, n4 = (max_tokens + 3) & ~3, (n + 4) & ~3
-    buf = torch.empty(3 * m4 + 2 * n4 + 8, dtype=torch.int32, device=lens.device)
-    p = buf.data_ptr()
-    lo, qs, nf, sl = 3 * m4, 3 * m4 + n4, 3 * m4 + 2 * n4, 3 * m4 + 2 * n4 + 4
+    # one allocation: slots, positions, seqs, q_start, lens, n_free, status
+    sizes = (max_tokens, max_tokens, max_tokens, n + 1, n, 1, 1)
+    slots, positions, seqs, q_start, lens_out, n_free_out, status = torch.empty(
+        3 * max_tokens + 2 * n + 3, dtype=torch.int32, device=lens.device).split_with_sizes(sizes)
+    q = q_start.data_ptr()  # (an empty part has no address)
+    p = q - 12 * max_tokens
     _call(dev, "pages_extend", lib.ifx_op_pages_extend, lens.data_ptr(), add.data_ptr(), n, table.data_ptr(),
-          table.shape[1], free.data_ptr(), free.numel(), n_free.data_ptr(), max_tokens, p + 4 * lo, p + 4 * nf,
-          p + 4 * qs, p, p + 4 * m4, p + 8 * m4, p + 4 * sl)
-    return PageStep(buf[lo:lo + n], buf[nf:nf + 1], buf[qs:qs + n + 1], buf[:max_tokens],
-                    buf[m4:m4 + max_tokens], buf[2 * m4:2 * m4 + max_tokens], buf[sl:sl + 1])
+          table.shape[1], free.data_ptr(), free.numel(), n_free.data_ptr(), max_tokens, q + 4 * n + 4, q + 8 * n + 4, q,
+          p, p + 4 * max_tokens, p + 8 * max_tokens, q + 8 * n + 8)
+    return PageStep(lens_out, n_free_out, q_start, slots, positions, seqs, status)
 
 
 def pages_release(done, lens, table, free, n_free):
@@ -233,18 +234,25 @@ def pages_release(done, lens, table, free, n_free):
     n = lens.numel()
     _need(table.dim() == 2 and table.shape[0] == n and done.numel() == n and n_free.numel() == 1,
           "pages_release shape mismatch")
-    lens_out, n_free_out = torch.empty_like(lens), torch.empty_like(n_free)
+    lens_out, n_free_out = torch.empty(n + 1, dtype=torch.int32, device=lens.device).split_with_sizes((n, 1))
+    p = n_free_out.data_ptr()
     _call(dev, "pages_release", lib.ifx_op_pages_release, done.data_ptr(), lens.data_ptr(), n, table.data_ptr(),
-          table.shape[1], free.data_ptr(), free.numel(), n_free.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr())
+          table.shape[1], free.data_ptr(), free.numel(), n_free.data_ptr(), p - 4 * n, p)
     return lens_out, n_free_out
 
 
+@lru_cache(maxsize=None)
 def kv4_page_bytes(n_kv_heads: int, head_dim: int) -> int:
     """Bytes of one page (64 rows of keys and values) of the cache in 4 bits."""
-    n = lib.ifx_kv4_page_bytes(n_kv_heads, head_dim)
+    n = lib.ifx_kv4_page_bytes(n_kv_heads, head_dim) if n_kv_heads > 0 and head_dim > 0 else 0
     if not n:
         raise IfxError(26, "kv4: 1 to 1024 kv heads, head_dim a multiple of 32 up to 256")
     return n
+
+
+@lru_cache(maxsize=None)
+def _workspace_bytes(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return lib.ifx_kv4_attention_workspace(n_heads, n_kv_heads, head_dim)
 
 
 def kv4_pages(n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
@@ -253,34 +261,37 @@ def kv4_pages(n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> to
 
 
 def _pool(what: str, pages: torch.Tensor, n_kv_heads: int, head_dim: int) -> int:
-    if pages.dtype != torch.uint8 or pages.dim() != 2 or not pages.is_contiguous():
+    if pages.dtype is not torch.uint8 or pages.dim() != 2 or not pages.is_contiguous():
         raise IfxError(24, f"{what}: pages must be a contiguous uint8 tensor [n_pages, page bytes]")
-    _need(pages.shape[1] == kv4_page_bytes(n_kv_heads, head_dim), f"{what}: page bytes mismatch")
-    return pages.shape[0]
+    n, size = pages.shape
+    if size != kv4_page_bytes(n_kv_heads, head_dim):
+        raise IfxError(20, f"{what}: page bytes mismatch")
+    return n
 
 
-def _rows(what: str, x: torch.Tensor) -> int:
-    """Stride between the rows of x [n, heads, head_dim], whose rows are contiguous."""
+def _rows(what: str, x: torch.Tensor):
+    """(rows, heads, head_dim, stride between the rows) of x, whose rows are contiguous."""
     if x.dtype not in _TYPES:
         raise IfxError(26, f"{what}: float32 or float16 rows")
-    _need(x.dim() == 3, f"{what}: expected [rows, heads, head_dim]")
+    if x.dim() != 3:
+        raise IfxError(20, f"{what}: expected [rows, heads, head_dim]")
     n, h, d = x.shape
-    if not x.numel():
-        return h * d
+    if x.is_contiguous():
+        return n, h, d, h * d
     sn, sh, sd = x.stride()
     if (sd != 1 and d != 1) or (sh != d and h != 1):
         raise IfxError(24, f"{what}: a row's heads must be contiguous")
-    return sn if n > 1 else h * d
+    return n, h, d, sn if n > 1 else h * d
 
 
 def kv4_store(k, v, slots, pages) -> None:
     """Rows k, v [n, n_kv_heads, head_dim] quantised into the rows slots [n] of
     the pages; a slot outside them (-1) skips its row. The slots differ."""
     dev = _dev(k, v, slots, pages)
-    ks, vs = _rows("kv4_store", k), _rows("kv4_store", v)
-    _need(k.shape == v.shape and k.dtype == v.dtype and slots.numel() == k.shape[0], "kv4_store shape mismatch")
+    n, g, d, ks = _rows("kv4_store", k)
+    vs = _rows("kv4_store", v)[3]
+    _need(k.shape == v.shape and k.dtype is v.dtype and slots.numel() == n, "kv4_store shape mismatch")
     _ints("kv4_store", slots)
-    n, g, d = k.shape
     np_ = _pool("kv4_store", pages, g, d)
     _call(dev, "kv4_store", lib.ifx_op_kv4_store, _TYPES[k.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
           slots.data_ptr(), n, pages.data_ptr(), np_, g, d)
@@ -312,35 +323,39 @@ def kv4_attention(q, pages, table, kv_len, n_kv_heads: int, q_start=None, scale=
     gives 0; rows of `out` behind the last sequence's stay as they were (a
     fresh `out` is zeroed when q_start is given). workspace: uint8 scratch kept
     by the caller (kv4_workspace), for one call at a time."""
-    qs = _rows("kv4_attention", q)
-    rows, h, d = q.shape
+    rows, h, d, qs = _rows("kv4_attention", q)
     n = kv_len.numel()
-    _need(n_kv_heads > 0 and h % n_kv_heads == 0, "kv4_attention: query heads must be a multiple of the kv heads")
+    if n_kv_heads <= 0 or h % n_kv_heads:
+        raise IfxError(20, "kv4_attention: query heads must be a multiple of the kv heads")
     np_ = _pool("kv4_attention", pages, n_kv_heads, d)
     _ints("kv4_attention", table, kv_len)
     _need(table.dim() == 2 and table.shape[0] == n, "kv4_attention: table is [n_seqs, max_pages]")
     _need(window >= 0, "kv4_attention: negative window")
+    starts = None
     if q_start is None:
         _need(rows == n, "kv4_attention: one row per sequence without q_start")
     else:
         _ints("kv4_attention", q_start)
         _need(q_start.numel() == n + 1, "kv4_attention: q_start is [n_seqs + 1]")
+        starts = q_start.data_ptr()
     if out is None:
-        out = (torch.empty if q_start is None else torch.zeros)(rows, h, d, dtype=q.dtype, device=q.device)
-    _need(out.shape == q.shape and out.dtype == q.dtype, "kv4_attention: out mismatch")
+        out, os = (torch.empty if starts is None else torch.zeros)((rows, h, d), dtype=q.dtype, device=q.device), h * d
+    else:
+        _need(out.shape == q.shape and out.dtype is q.dtype, "kv4_attention: out mismatch")
+        os = _rows("kv4_attention", out)[3]
     if workspace is None:
-        workspace = kv4_workspace(h, n_kv_heads, d, q.device)
-    dev = _dev(q, pages, table, kv_len, out, workspace, *(() if q_start is None else (q_start,)))
+        workspace = torch.empty(_workspace_bytes(h, n_kv_heads, d), dtype=torch.uint8, device=q.device)
+    dev = _dev(q, pages, table, kv_len, out, workspace) if q_start is None else _dev(
+        q, pages, table, kv_len, out, workspace, q_start)
     _call(dev, "kv4_attention", lib.ifx_op_kv4_attention, _TYPES[q.dtype], q.data_ptr(), qs, rows, pages.data_ptr(),
-          np_, table.data_ptr(), table.shape[1], kv_len.data_ptr(), None if q_start is None else q_start.data_ptr(),
-          n, h, n_kv_heads, d, d ** -0.5 if scale is None else scale, window, out.data_ptr(),
-          _rows("kv4_attention", out), workspace.data_ptr(), workspace.numel())
+          np_, table.data_ptr(), table.shape[1], kv_len.data_ptr(), starts, n, h, n_kv_heads, d,
+          d ** -0.5 if scale is None else scale, window, out.data_ptr(), os, workspace.data_ptr(), workspace.numel())
     return out
 
 
 def kv4_workspace(n_heads: int, n_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
     """Scratch of kv4_attention for these shapes."""
-    return torch.empty(lib.ifx_kv4_attention_workspace(n_heads, n_kv_heads, head_dim), dtype=torch.uint8, device=device)
+    return torch.empty(_workspace_bytes(n_heads, n_kv_heads, head_dim), dtype=torch.uint8, device=device)
 
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
