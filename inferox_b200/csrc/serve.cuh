@@ -101,6 +101,7 @@ struct Kv4AttnArgs {
   int max_pages, n_seqs, H, G, hd, window;
   float scale;
   void *ws;
+  bool alone = false;         // set by the launch: a CTA per segment
 };
 ifx_status op_kv4_attention(const Kv4AttnArgs &a, cudaStream_t st);
 // Bytes of scratch a call with these shapes needs.
