@@ -1131,19 +1131,10 @@ __global__ void __launch_bounds__(kChunkThreads, ChunkSmem<NB>::kPerSm) kv4_attn
       base[0] -= (float)pf;
       base[1] -= (float)pf;
       float sum[2] = {0.f, 0.f};
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      // ---- probabilities
+      uint32_t ph[4][4], pl[4][4];
 #pragma unroll
-        for (int i = 0; i < 4 * NB; ++i) {
-          o[i][0] *= alpha[0];
-          o[i][1] *= alpha[0];
-          o[i][2] *= alpha[1];
-          o[i][3] *= alpha[1];
-        }
-      }
-      // ---- output
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        uint32_t ph[4], pl[4];
+      for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -1152,11 +1143,19 @@ __global__ void __launch_bounds__(kChunkThreads, ChunkSmem<NB>::kPerSm) kv4_attn
             const float x1 = ex2(fmaf(sc[2 * ks + k][2 * i + 1], qs[i], -base[i]));
             sum[i] += x0 + x1;
             const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
-            ph[2 * k + i] = h2(__floats2half2_rn(h0, h1));  // the first 11 bits, exactly
-            pl[2 * k + i] = h2(__floats2half2_rn(x0 - h0, x1 - h1));
+            ph[ks][2 * k + i] = h2(__floats2half2_rn(h0, h1));  // the first 11 bits, exactly
+            pl[ks][2 * k + i] = h2(__floats2half2_rn(x0 - h0, x1 - h1));
           }
+      // ---- output: a page's sum starts from zero and is added in f32, whose
+      // rounding has no direction (the tensor cores cut their sums off: 40
+      // pages in one accumulator came out 4.8e-6 off, so 4e-7)
 #pragma unroll
-        for (int n = 0; n < 4 * NB; n += 4) {
+      for (int n = 0; n < 4 * NB; n += 4) {
+        float acc[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
           uint32_t vh[2][4], vl[2][4];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -1165,12 +1164,16 @@ __global__ void __launch_bounds__(kChunkThreads, ChunkSmem<NB>::kPerSm) kv4_attn
             ldsm_x4_t(vl[q], smem_u32(Vl + at));
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816(o[n + k], pl[0], pl[1], pl[2], pl[3], vh[k >> 1][2 * (k & 1)], vh[k >> 1][2 * (k & 1) + 1], o[n + k]);
+          for (int k = 0; k < 4; ++k) mma_16816(acc[k], pl[ks][0], pl[ks][1], pl[ks][2], pl[ks][3], vh[k >> 1][2 * (k & 1)], vh[k >> 1][2 * (k & 1) + 1], acc[k]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816(o[n + k], ph[0], ph[1], ph[2], ph[3], vl[k >> 1][2 * (k & 1)], vl[k >> 1][2 * (k & 1) + 1], o[n + k]);
+          for (int k = 0; k < 4; ++k) mma_16816(acc[k], ph[ks][0], ph[ks][1], ph[ks][2], ph[ks][3], vl[k >> 1][2 * (k & 1)], vl[k >> 1][2 * (k & 1) + 1], acc[k]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816(o[n + k], ph[0], ph[1], ph[2], ph[3], vh[k >> 1][2 * (k & 1)], vh[k >> 1][2 * (k & 1) + 1], o[n + k]);
+          for (int k = 0; k < 4; ++k) mma_16816(acc[k], ph[ks][0], ph[ks][1], ph[ks][2], ph[ks][3], vh[k >> 1][2 * (k & 1)], vh[k >> 1][2 * (k & 1) + 1], acc[k]);
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n + k][i] = fmaf(o[n + k][i], alpha[i >> 1], acc[k][i]);
       }
       const float back = __uint_as_float((uint32_t)(127 - pf) << 23);
       l[0] = fmaf(sum[0], back, l[0]);
