@@ -202,6 +202,15 @@ void ifx_kv_batch_free(ifx_kv_batch *kb);
  * most 4096. Results are those of ifx_kv_batch_create's batch. */
 ifx_status ifx_kv_batch_create_paged(ifx_model *m, size_t max_seq_len, int batch,
                                      size_t n_pages, ifx_kv_batch **out);
+/* No reference counterpart: a paged batch whose cache is held in 4 bits (the
+ * pages of ifx_op_kv4_store, one table for all layers; 4.5 bits a value
+ * against 16). Keys and values of a prompt and of every step are quantised
+ * as they are stored, so decode steps see the quantised rows; attention
+ * within a prompt uses its rows as computed. head_dim 32, 64, 96 or 128; no
+ * bound on max_seq_len but the pool. Otherwise as
+ * ifx_kv_batch_create_paged. */
+ifx_status ifx_kv_batch_create_q4(ifx_model *m, size_t max_seq_len, int batch,
+                                  size_t n_pages, ifx_kv_batch **out);
 /* Pages of a paged batch that no sequence holds, and the pool size (both 0
  * for a batch made by ifx_kv_batch_create). */
 ifx_status ifx_kv_batch_pages(const ifx_kv_batch *kb, size_t *free_pages,
@@ -250,6 +259,17 @@ typedef struct ifx_sampler {
  * counter-based Philox uniform from (seed, offset). */
 ifx_status ifx_sample(ifx_model *m, const ifx_sampler *s, uint64_t seed,
                       uint64_t offset, uint32_t *token_out);
+
+/* Sampler::sample's rule (sampler.rs:28-73) for rows 0 .. n-1 of the latest
+ * logits on the device: those of kb's latest decode step (row i is the
+ * caller's row i), or of its latest prompt's last row (n = 1); kb NULL: the
+ * model's latest logits (n = 1). Each row has its own settings s[i], min_p[i]
+ * (nullable: none) and draw u[i] in [0, 1), as ifx_op_sample_rows describes.
+ * tokens [n] (0xffffffff where every logit is masked); logprobs [n] is
+ * nullable. Host buffers; returns when the tokens are there. */
+ifx_status ifx_sample_batch(ifx_model *m, ifx_kv_batch *kb, int n,
+                            const ifx_sampler *s, const float *min_p,
+                            const float *u, uint32_t *tokens, float *logprobs);
 
 /* ------------------------- op-level entry points ------------------------ */
 /* dequantize_f32 (src/gguf/dequant.rs:10-31): bit-exact with the

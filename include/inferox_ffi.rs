@@ -78,6 +78,11 @@ extern "C" {
                                out: *mut *mut IfxKvBatch) -> c_int;
     pub fn ifx_kv_batch_create_paged(m: *mut IfxModel, max_seq: usize, batch: c_int,
                                      n_pages: usize, out: *mut *mut IfxKvBatch) -> c_int;
+    pub fn ifx_kv_batch_create_q4(m: *mut IfxModel, max_seq: usize, batch: c_int, n_pages: usize,
+                                  out: *mut *mut IfxKvBatch) -> c_int;
+    pub fn ifx_sample_batch(m: *mut IfxModel, kb: *mut IfxKvBatch, n: c_int, s: *const IfxSampler,
+                            min_p: *const f32, u: *const f32, tokens: *mut u32,
+                            logprobs: *mut f32) -> c_int;
     pub fn ifx_kv_batch_pages(kb: *const IfxKvBatch, free_pages: *mut usize,
                               total_pages: *mut usize) -> c_int;
     pub fn ifx_kv_batch_free(kb: *mut IfxKvBatch);

@@ -111,6 +111,8 @@ def _load():
         "ifx_bench_kernel": (st, [vp, vp, C.c_char_p, C.c_int, fp, C.POINTER(C.c_uint64)]),
         "ifx_kv_batch_create": (st, [vp, sz, C.c_int, C.POINTER(vp)]),
         "ifx_kv_batch_create_paged": (st, [vp, sz, C.c_int, sz, C.POINTER(vp)]),
+        "ifx_kv_batch_create_q4": (st, [vp, sz, C.c_int, sz, C.POINTER(vp)]),
+        "ifx_sample_batch": (st, [vp, vp, C.c_int, C.POINTER(SamplerC), fp, fp, u32p, fp]),
         "ifx_kv_batch_pages": (st, [vp, C.POINTER(sz), C.POINTER(sz)]),
         "ifx_kv_batch_free": (None, [vp]),
         "ifx_kv_batch_len": (st, [vp, C.c_int, C.POINTER(sz)]),

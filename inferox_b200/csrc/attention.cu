@@ -1328,6 +1328,23 @@ static ifx_status launch_prefill_tc(const PrefillAttnArgs &a, cudaStream_t st) {
   return IFX_OK;
 }
 
+__global__ void rope_rows_kernel(float *x, int64_t stride, int heads, int hd, int rope_dim, float base, const int *pos) {
+  float *row = x + blockIdx.x * stride;
+  const int at = pos[blockIdx.x], pairs = rope_dim / 2;
+  for (int e = threadIdx.x; e < heads * pairs; e += blockDim.x) {
+    float *v = row + (int64_t)(e / pairs) * hd + 2 * (e % pairs);
+    rope_pair(v[0], v[1], 2 * (e % pairs), rope_dim, base, at);
+  }
+}
+
+ifx_status op_rope_rows(float *x, int64_t stride, int rows, int heads, int hd, int rope_dim, float base, const int *pos,
+                        cudaStream_t st) {
+  if (rows < 1 || rope_dim < 2) return IFX_OK;
+  rope_rows_kernel<<<(unsigned)rows, 256, 0, st>>>(x, stride, heads, hd, rope_dim, base, pos);
+  IFX_CUDA(cudaGetLastError());
+  return IFX_OK;
+}
+
 ifx_status prefill_attention(const PrefillAttnArgs &a, cudaStream_t st) {
   // causal prefill into a cache: the streamed kernel (8 warps = the kv
   // head's query heads x row tiles)

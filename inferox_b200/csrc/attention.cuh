@@ -64,4 +64,9 @@ struct PrefillAttnArgs {
 };
 ifx_status prefill_attention(const PrefillAttnArgs &a, cudaStream_t st);
 
+// RoPE of the first `heads` heads of every row of x (rows `stride` apart) at
+// the row's own position (the rotation of decode_attention).
+ifx_status op_rope_rows(float *x, int64_t stride, int rows, int heads, int hd, int rope_dim, float base, const int *pos,
+                        cudaStream_t st);
+
 }  // namespace ifx

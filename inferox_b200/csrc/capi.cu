@@ -248,9 +248,25 @@ ifx_status ifx_kv_batch_create_paged(ifx_model *m, size_t max_seq_len, int batch
   IFX_GUARD({ return kv_batch_create(m, max_seq_len, batch, n_pages, out); })
 }
 
+ifx_status ifx_kv_batch_create_q4(ifx_model *m, size_t max_seq_len, int batch, size_t n_pages,
+                                  ifx_kv_batch **out) {
+  if (!m || !out || !max_seq_len || !n_pages || n_pages > (size_t)INT32_MAX)
+    return fail(IFX_ERR_INVALID_ARGUMENT, "kv_batch_create_q4: bad argument");
+  IFX_GUARD({
+    ifx_kv_batch *kb = new ifx_kv_batch();
+    const ifx_status s = kb->kb.create_q4(&m->m, max_seq_len, batch, n_pages);
+    if (s != IFX_OK) {
+      delete kb;
+      return s;
+    }
+    *out = kb;
+    return IFX_OK;
+  })
+}
+
 ifx_status ifx_kv_batch_pages(const ifx_kv_batch *kb, size_t *free_pages, size_t *total_pages) {
   if (!kb || !free_pages || !total_pages) return fail(IFX_ERR_INVALID_ARGUMENT, "kv_batch_pages: null argument");
-  *free_pages = kb->kb.free_pages.size();
+  *free_pages = kb->kb.q4 ? kb->kb.n_free : kb->kb.free_pages.size();
   *total_pages = kb->kb.n_pages;
   return IFX_OK;
 }
@@ -298,6 +314,13 @@ ifx_status ifx_decode_greedy_batch(ifx_model *m, ifx_kv_batch *kb, const uint32_
   if (!m || !kb || !tokens) return fail(IFX_ERR_INVALID_ARGUMENT, "decode_greedy_batch: null argument");
   if (kb->kb.m != &m->m) return fail(IFX_ERR_INVALID_ARGUMENT, "decode_greedy_batch: batch belongs to another model");
   IFX_GUARD({ return m->m.decode_greedy_batch(kb->kb, tokens, n_steps, out_tokens, device_ms); })
+}
+
+ifx_status ifx_sample_batch(ifx_model *m, ifx_kv_batch *kb, int n, const ifx_sampler *s, const float *min_p,
+                            const float *u, uint32_t *tokens, float *logprobs) {
+  if (!m || !s || !u || !tokens) return fail(IFX_ERR_INVALID_ARGUMENT, "sample_batch: null argument");
+  if (kb && kb->kb.m != &m->m) return fail(IFX_ERR_INVALID_ARGUMENT, "sample_batch: batch belongs to another model");
+  IFX_GUARD({ return m->m.sample_batch(kb ? &kb->kb : nullptr, n, s, min_p, u, tokens, logprobs); })
 }
 
 ifx_status ifx_bench_kernel(ifx_model *m, ifx_kv *kv, const char *which, int reps,

@@ -27,6 +27,7 @@
 #include "gemm.cuh"
 #include "gemv.cuh"
 #include "kquant.h"
+#include "serve.cuh"
 #include "nvtx3/nvToolsExt.h"
 #include "gguf.h"
 #include "model.h"
@@ -517,6 +518,7 @@ Model::~Model() {
     F(L.ffn_norm);
     for (QMatrix *q : {&L.wq, &L.wk, &L.wv, &L.wo, &L.w1, &L.w3, &L.w2}) F(q->d);
   }
+  F(sample_buf);
   F(out_w.d);
   F(out_norm);
   F(emb_raw);
@@ -599,8 +601,6 @@ ifx_status KvBatch::create(Model *model, size_t max_seq_len, int nseq, size_t pa
     ns = std::min(ns, 64);
     while (ns < 64 && decode_attention_smem(grp, hd, (int)max_seq, ns) > 160 * 1024) ++ns;
   }
-  const size_t D = c.hidden_size, F = m->Fl, V = c.vocab_size;
-  const size_t qkvw = (size_t)(H + 2 * G) * hd;
   dev = m->device;
   IFX_CUDA(cudaSetDevice(m->device));
   const size_t cache = paged ? (size_t)page_stride * n_pages : per_layer * c.n_layers * nseq;
@@ -612,6 +612,17 @@ ifx_status KvBatch::create(Model *model, size_t max_seq_len, int nseq, size_t pa
     free_pages.clear();
     for (size_t i = n_pages; i-- > 0;) free_pages.push_back((int)i);  // page 0 handed out first
   }
+  IFX_TRY(dalloc(&part_o, (size_t)nseq * H * ns * hd));
+  IFX_TRY(dalloc(&part_ml, (size_t)nseq * H * ns));
+  IFX_TRY(dalloc(&counters, (size_t)nseq * G));
+  return common(c, nseq);
+}
+
+// The step's workspace, whatever the cache.
+ifx_status KvBatch::common(const ifx_config &c, int nseq) {
+  const int G = (int)m->Gl, H = (int)m->Hl, hd = (int)c.head_dim;
+  const size_t D = c.hidden_size, F = m->Fl, V = c.vocab_size;
+  const size_t qkvw = (size_t)(H + 2 * G) * hd;
   IFX_TRY(dalloc(&pos, (size_t)nseq));
   IFX_TRY(dalloc(&x, nseq * D));
   IFX_TRY(dalloc(&qkv, nseq * qkvw));
@@ -619,9 +630,6 @@ ifx_status KvBatch::create(Model *model, size_t max_seq_len, int nseq, size_t pa
   IFX_TRY(dalloc(&gate, nseq * F));
   IFX_TRY(dalloc(&up, nseq * F));
   IFX_TRY(dalloc(&logits, nseq * V));
-  IFX_TRY(dalloc(&part_o, (size_t)nseq * H * ns * hd));
-  IFX_TRY(dalloc(&part_ml, (size_t)nseq * H * ns));
-  IFX_TRY(dalloc(&counters, (size_t)nseq * G));
   IFX_TRY(dalloc(&ids, (size_t)nseq));
   IFX_TRY(dalloc(&out, (size_t)nseq));
   IFX_TRY(dalloc(&keys, (size_t)nseq));
@@ -633,13 +641,89 @@ ifx_status KvBatch::create(Model *model, size_t max_seq_len, int nseq, size_t pa
   return IFX_OK;
 }
 
+ifx_status KvBatch::create_q4(Model *model, size_t max_seq_len, int nseq, size_t pages) {
+  m = model;
+  batch = nseq;
+  max_seq = max_seq_len;
+  const ifx_config &c = m->cfg;
+  if (m->tp > 1) return fail(IFX_ERR_UNSUPPORTED, "batched decode: tensor parallelism not supported");
+  if (nseq < 1 || nseq > kGemmSmallMax)
+    return fail(IFX_ERR_INVALID_ARGUMENT, "batched decode: 1 to 32 sequences");
+  const int G = (int)m->Gl, H = (int)m->Hl, hd = (int)c.head_dim;
+  if (!kv4_head_dim_ok((size_t)hd) || hd > 128)
+    return fail(IFX_ERR_UNSUPPORTED, "4-bit cache: head_dim must be 32, 64, 96 or 128");
+  const size_t most = (size_t)INT32_MAX / kKv4PageRows;
+  if (pages > most || max_seq > (size_t)INT32_MAX - kKv4PageRows)
+    return fail(IFX_ERR_INVALID_ARGUMENT, "4-bit cache: too many pages for 32-bit slots");
+  q4 = true;
+  page_rows = kKv4PageRows;
+  max_pages = (int)((max_seq + kKv4PageRows - 1) / kKv4PageRows);
+  n_pages = n_free = pages;
+  layer_bytes = (int64_t)(kv4_page_bytes((size_t)G, (size_t)hd) * pages);
+  dev = m->device;
+  IFX_CUDA(cudaSetDevice(m->device));
+  IFX_TRY(dalloc(&pages4, (size_t)layer_bytes * c.n_layers));
+  IFX_TRY(dalloc(&table_dev, (size_t)nseq * max_pages));
+  IFX_TRY(dalloc(&free4, pages));
+  IFX_TRY(dalloc(&n_free4, 1));
+  IFX_TRY(dalloc(&add4, (size_t)nseq));
+  IFX_TRY(dalloc(&ones4, (size_t)nseq));
+  IFX_TRY(dalloc(&lens4, 2 * (size_t)nseq + 3));
+  const size_t rows = std::max(max_seq, (size_t)nseq);
+  IFX_TRY(dalloc(&slots4, rows));
+  IFX_TRY(dalloc(&positions4, rows));
+  ws4_bytes = kv4_attention_ws(H, G, hd);
+  uint8_t *w = nullptr;
+  IFX_TRY(dalloc(&w, ws4_bytes));
+  ws4 = w;
+  std::vector<int> ids_(pages), one((size_t)nseq, 1);
+  for (size_t i = 0; i < pages; ++i) ids_[i] = (int)(pages - 1 - i);  // page 0 handed out first
+  const int n = (int)pages;
+  IFX_CUDA(cudaMemcpy(free4, ids_.data(), pages * sizeof(int), cudaMemcpyHostToDevice));
+  IFX_CUDA(cudaMemcpy(n_free4, &n, sizeof(int), cudaMemcpyHostToDevice));
+  IFX_CUDA(cudaMemcpy(ones4, one.data(), (size_t)nseq * sizeof(int), cudaMemcpyHostToDevice));
+  held.assign((size_t)nseq, 0);
+  return common(c, nseq);
+}
+
+ifx_status KvBatch::take(const int *seqs, int n, size_t rows) {
+  size_t need = 0;
+  auto pages_of = [&](int b) { return (int)((len[(size_t)b] + rows + page_rows - 1) / page_rows); };
+  for (int i = 0; i < n; ++i) {
+    const int b = seqs ? seqs[i] : i;
+    if (len[(size_t)b] + rows > max_seq) return fail(IFX_ERR_INVALID_TENSOR_INDEX, "KV cache is full");
+    need += (size_t)std::max(0, pages_of(b) - held[(size_t)b]);
+  }
+  if (need > n_free)
+    return fail(IFX_ERR_OUT_OF_MEMORY, "paged batch: the page pool is exhausted (" +
+                                           std::to_string(n_pages) + " pages)");
+  n_free -= need;
+  for (int i = 0; i < n; ++i) {
+    const int b = seqs ? seqs[i] : i;
+    held[(size_t)b] = std::max(held[(size_t)b], pages_of(b));
+  }
+  return IFX_OK;
+}
+
+// Pages and slots of the step's rows (add[b] of each sequence) behind the
+// lengths in pos; lens4 holds the lengths with them.
+ifx_status KvBatch::extend(const int *add, size_t max_tokens, cudaStream_t st) {
+  int *nf = lens4 + batch, *qs = nf + 1, *status = qs + batch + 1;
+  PagesExtendArgs e{pos, add, batch, table_dev, max_pages, free4, (int)n_pages, n_free4, (int64_t)max_tokens,
+                    lens4, nf, qs, slots4, positions4, nullptr, status};
+  IFX_TRY(op_pages_extend(e, st));
+  IFX_CUDA(cudaMemcpyAsync(n_free4, nf, sizeof(int), cudaMemcpyDeviceToDevice, st));
+  return IFX_OK;
+}
+
 KvBatch::~KvBatch() {
   if (dev >= 0) cudaSetDevice(dev);
   if (graph) cudaGraphExecDestroy(graph);
   for (void *p : {(void *)k, (void *)v, (void *)pos, (void *)x, (void *)qkv, (void *)attn,
                   (void *)gate, (void *)up, (void *)logits, (void *)part_o, (void *)part_ml,
                   (void *)counters, (void *)xf, (void *)ids, (void *)out, (void *)keys,
-                  (void *)slots, (void *)table_dev})
+                  (void *)slots, (void *)table_dev, (void *)pages4, (void *)free4, (void *)n_free4,
+                  (void *)add4, (void *)ones4, (void *)lens4, (void *)slots4, (void *)positions4, ws4})
     if (p) cudaFree(p);
 }
 
@@ -661,6 +745,12 @@ ifx_status KvBatch::reserve(int seq, size_t rows, cudaStream_t st) {
   IFX_CUDA(cudaMemcpyAsync(table_dev + (size_t)seq * max_pages + have, row + have,
                            sizeof(int) * (size_t)(need - have), cudaMemcpyHostToDevice, st));
   return IFX_OK;
+}
+
+void KvBatch::latest_rows(int n) {
+  order.resize((size_t)n);
+  for (int i = 0; i < n; ++i) order[(size_t)i] = i;
+  after_prompt = false;
 }
 
 void KvBatch::release(int seq) {
@@ -1062,7 +1152,20 @@ ifx_status Model::prefill_seq(KvBatch &kb, int seq, const uint32_t *ids, size_t 
   view.m = this;
   view.max_seq = kb.max_seq;
   view.per_layer = kb.per_layer;
-  if (kb.paged) {
+  std::vector<int> add;
+  if (kb.q4) {
+    for (size_t i = 0; i < n; ++i)
+      if (ids[i] >= cfg.vocab_size) return fail(IFX_ERR_INVALID_TENSOR_INDEX, "tensor index out of bounds: 0");
+    if (n == 0) return IFX_OK;
+    IFX_CUDA(cudaSetDevice(device));
+    IFX_TRY(ensure_ws(n));
+    IFX_TRY(kb.take(&seq, 1, n));
+    add.assign((size_t)kb.batch, 0);
+    add[(size_t)seq] = (int)n;
+    IFX_CUDA(cudaMemcpyAsync(kb.add4, add.data(), sizeof(int) * kb.batch, cudaMemcpyHostToDevice, stream));
+    IFX_TRY(kb.extend(kb.add4, n, stream));
+    view.q4 = &kb;
+  } else if (kb.paged) {
     if (kb.len[(size_t)seq] + n > kb.max_seq)
       return fail(IFX_ERR_INVALID_TENSOR_INDEX, "KV cache is full");
     IFX_CUDA(cudaSetDevice(device));
@@ -1080,6 +1183,8 @@ ifx_status Model::prefill_seq(KvBatch &kb, int seq, const uint32_t *ids, size_t 
   view.len = kb.len[(size_t)seq];
   view.mega_tried = true;  // never planned for the persistent kernel
   const ifx_status s = run_prompt(&view, ids, n, logits_host, last_row_only);
+  kb.order.assign(1, 0);
+  kb.after_prompt = true;
   kb.len[(size_t)seq] = view.len;
   return s;
 }
@@ -1098,6 +1203,8 @@ ifx_status Model::enqueue_decode_batch(KvBatch &kb, cudaStream_t st, int n, cons
   const float eps = c.norm_eps;
   embed_rows_kernel<<<(unsigned)B, 256, 0, st>>>(emb_raw, emb_type, D, kb.ids, kb.x);
   IFX_CUDA(cudaGetLastError());
+  // one table, one set of slots and positions for all layers
+  if (kb.q4) IFX_TRY(kb.extend(slot_dev ? kb.add4 : kb.ones4, (size_t)B, st));
   for (uint64_t l = 0; l < c.n_layers; ++l) {
     Layer &L = layers[l];
     StageZero zq;  // the QKV GEMMs accumulate into qkv
@@ -1110,35 +1217,65 @@ ifx_status Model::enqueue_decode_batch(KvBatch &kb, cudaStream_t st, int n, cons
       const int64_t ls[3] = {qkvw, qkvw, qkvw};
       IFX_TRY(gemm_small_run_multi(ws, cs, ls, 3, kb.xf, B, err, st));
     }
-    DecodeAttnArgs a{};
-    a.qkv = kb.qkv;
-    a.qkv_stride = qkvw;
-    a.kc = kb.k + l * kb.per_layer;
-    a.vc = kb.v + l * kb.per_layer;
-    a.kv_seq_stride = kb.paged ? 0 : (int64_t)(c.n_layers * kb.per_layer);
-    if (kb.paged) {
-      a.page_table = kb.table_dev;
-      a.page_rows = kb.page_rows;
+    if (kb.q4) {
+      // rows into the cache in 4 bits, then attention over it; RoPE at
+      // position 0 is the identity (forward.rs:371-372)
+      if (!opts.rope_compat)
+        IFX_TRY(op_rope_rows(kb.qkv, qkvw, B, H + G, hd, (int)c.rope_dim, c.rope_base, kb.positions4, st));
+      Kv4RowsArgs r{kb.qkv + Hh, kb.qkv + Hh + G * hd, nullptr, nullptr, IFX_TYPE_F32, B, qkvw, qkvw,
+                    kb.slots4, kb.pages4 + l * kb.layer_bytes, (int64_t)kb.n_pages, G, hd};
+      IFX_TRY(op_kv4_store(r, st));
+      Kv4AttnArgs a{};
+      a.q = kb.qkv;
+      a.out = kb.attn;
+      a.type = IFX_TYPE_F32;
+      a.q_stride = qkvw;
+      a.out_stride = Hh;
+      a.rows = B;
+      a.pages = r.pages;
+      a.n_pages = r.n_pages;
+      a.table = kb.table_dev;
+      a.kv_len = kb.lens4;
+      a.q_start = slot_dev ? kb.lens4 + kb.batch + 1 : nullptr;
       a.max_pages = kb.max_pages;
-      a.page_stride = kb.page_stride;
+      a.n_seqs = kb.batch;
+      a.H = H;
+      a.G = G;
+      a.hd = hd;
+      a.scale = 1.0f / sqrtf((float)hd);
+      a.ws = kb.ws4;
+      IFX_TRY(op_kv4_attention(a, st));
+    } else {
+      DecodeAttnArgs a{};
+      a.qkv = kb.qkv;
+      a.qkv_stride = qkvw;
+      a.kc = kb.k + l * kb.per_layer;
+      a.vc = kb.v + l * kb.per_layer;
+      a.kv_seq_stride = kb.paged ? 0 : (int64_t)(c.n_layers * kb.per_layer);
+      if (kb.paged) {
+        a.page_table = kb.table_dev;
+        a.page_rows = kb.page_rows;
+        a.max_pages = kb.max_pages;
+        a.page_stride = kb.page_stride;
+      }
+      a.pos = kb.pos;
+      a.part_o = kb.part_o;
+      a.part_ml = kb.part_ml;
+      a.counters = kb.counters;
+      a.attn_out = kb.attn;
+      a.H = H;
+      a.G = G;
+      a.hd = hd;
+      a.max_seq = (int)kb.max_seq;
+      a.ns = kb.ns;
+      a.rope_compat = opts.rope_compat;
+      a.rope_dim = (int)c.rope_dim;
+      a.rope_base = c.rope_base;
+      a.err = err;
+      a.batch = B;
+      a.slot = slot_dev;
+      IFX_TRY(decode_attention(a, st, true));
     }
-    a.pos = kb.pos;
-    a.part_o = kb.part_o;
-    a.part_ml = kb.part_ml;
-    a.counters = kb.counters;
-    a.attn_out = kb.attn;
-    a.H = H;
-    a.G = G;
-    a.hd = hd;
-    a.max_seq = (int)kb.max_seq;
-    a.ns = kb.ns;
-    a.rope_compat = opts.rope_compat;
-    a.rope_dim = (int)c.rope_dim;
-    a.rope_base = c.rope_base;
-    a.err = err;
-    a.batch = B;
-    a.slot = slot_dev;
-    IFX_TRY(decode_attention(a, st, true));
     IFX_TRY(stage_small(kb.attn, nullptr, nullptr, 0.f, GX_PLAIN, B, Hh, kb.xf, st));
     IFX_TRY(gemm_small_run(L.wo, kb.xf, B, kb.x, D, err, st));  // x += attn Wo^T
     StageZero zf;  // W1 / W3 accumulate into gate / up
@@ -1178,8 +1315,10 @@ ifx_status Model::decode_batch(KvBatch &kb, const uint32_t *tokens, float *logit
   }
   IFX_CUDA(cudaSetDevice(device));
   cudaStream_t st = stream;
+  if (kb.q4) IFX_TRY(kb.take(nullptr, kb.batch, 1));
   for (int b = 0; b < kb.batch; ++b) IFX_TRY(kb.reserve(b, kb.len[(size_t)b] + 1, st));
   IFX_CUDA(cudaMemcpyAsync(kb.ids, tokens, sizeof(uint32_t) * kb.batch, cudaMemcpyHostToDevice, st));
+  kb.latest_rows(kb.batch);
   IFX_TRY(enqueue_decode_batch(kb, st));
   if (logits_host)
     IFX_CUDA(cudaMemcpyAsync(logits_host, kb.logits, sizeof(float) * kb.batch * cfg.vocab_size,
@@ -1211,18 +1350,86 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
   }
   IFX_CUDA(cudaSetDevice(device));
   cudaStream_t st = stream;
+  kb.latest_rows(n);
+  std::vector<int> sorted_seqs, add;
+  std::vector<uint32_t> sorted_tokens, sorted_out;
+  if (kb.q4) {
+    // the device lays rows out by sequence: the step runs in that order, and
+    // row i of the results is put back to seqs[i]
+    IFX_TRY(kb.take(seqs, n, 1));
+    std::vector<int> at((size_t)n);
+    for (int i = 0; i < n; ++i) at[(size_t)i] = i;
+    std::sort(at.begin(), at.end(), [&](int x, int y) { return seqs[x] < seqs[y]; });
+    add.assign((size_t)kb.batch, 0);
+    for (int i = 0; i < n; ++i) {
+      sorted_seqs.push_back(seqs[at[(size_t)i]]);
+      sorted_tokens.push_back(tokens[at[(size_t)i]]);
+      kb.order[(size_t)at[(size_t)i]] = i;
+      add[(size_t)seqs[i]] = 1;
+    }
+    IFX_CUDA(cudaMemcpyAsync(kb.add4, add.data(), sizeof(int) * kb.batch, cudaMemcpyHostToDevice, st));
+  }
+  const int *run_seqs = kb.q4 ? sorted_seqs.data() : seqs;
+  const uint32_t *run_tokens = kb.q4 ? sorted_tokens.data() : tokens;
   for (int i = 0; i < n; ++i) IFX_TRY(kb.reserve(seqs[i], kb.len[(size_t)seqs[i]] + 1, st));
-  IFX_CUDA(cudaMemcpyAsync(kb.ids, tokens, sizeof(uint32_t) * n, cudaMemcpyHostToDevice, st));
-  IFX_CUDA(cudaMemcpyAsync(kb.slots, seqs, sizeof(int) * n, cudaMemcpyHostToDevice, st));
+  IFX_CUDA(cudaMemcpyAsync(kb.ids, run_tokens, sizeof(uint32_t) * n, cudaMemcpyHostToDevice, st));
+  IFX_CUDA(cudaMemcpyAsync(kb.slots, run_seqs, sizeof(int) * n, cudaMemcpyHostToDevice, st));
   IFX_TRY(enqueue_decode_batch(kb, st, n, kb.slots));
-  if (logits_host)
+  if (logits_host && !kb.q4)
     IFX_CUDA(cudaMemcpyAsync(logits_host, kb.logits, sizeof(float) * n * cfg.vocab_size,
                              cudaMemcpyDeviceToHost, st));
-  if (argmax_host)
-    IFX_CUDA(cudaMemcpyAsync(argmax_host, kb.out, sizeof(uint32_t) * n, cudaMemcpyDeviceToHost, st));
+  for (int i = 0; logits_host && kb.q4 && i < n; ++i)
+    IFX_CUDA(cudaMemcpyAsync(logits_host + (size_t)i * cfg.vocab_size,
+                             kb.logits + (size_t)kb.order[(size_t)i] * cfg.vocab_size,
+                             sizeof(float) * cfg.vocab_size, cudaMemcpyDeviceToHost, st));
+  if (argmax_host) {
+    sorted_out.resize((size_t)n);
+    IFX_CUDA(cudaMemcpyAsync(sorted_out.data(), kb.out, sizeof(uint32_t) * n, cudaMemcpyDeviceToHost, st));
+  }
   IFX_CUDA(cudaStreamSynchronize(st));
+  for (int i = 0; argmax_host && i < n; ++i) argmax_host[i] = sorted_out[(size_t)kb.order[(size_t)i]];
   for (int i = 0; i < n; ++i) kb.len[(size_t)seqs[i]] += 1;
   return check_err();
+}
+
+// Draws for rows 0..n-1 of the latest logits: row-wise sampling (op_sample_rows)
+// with every row's own settings. The settings travel in one copy.
+ifx_status Model::sample_batch(KvBatch *kb, int n, const ifx_sampler *s, const float *min_p, const float *u,
+                               uint32_t *tokens, float *logprobs) {
+  NvtxRange nvtx_("ifx:sample_batch");
+  const bool of_model = !kb || kb->after_prompt;
+  const int rows = kb ? (int)kb->order.size() : 1;
+  if (n < 1 || n > (of_model ? 1 : rows))
+    return fail(IFX_ERR_INVALID_ARGUMENT, "sample_batch: no such row in the latest logits");
+  IFX_CUDA(cudaSetDevice(device));
+  constexpr int W = 7;  // u, temperature, top_k, top_p, min_p; token, logprob
+  if (!sample_buf) IFX_TRY(dalloc(&sample_buf, (size_t)W * kGemmSmallMax));
+  cudaStream_t st = stream;
+  std::vector<float> in((size_t)5 * rows, 0.f), out((size_t)2 * rows);
+  for (int r = 0; r < rows; ++r) in[(size_t)(3 * rows + r)] = 1.f;  // rows not asked for: greedy
+  for (int i = 0; i < n; ++i) {
+    const int r = of_model ? 0 : kb->order[(size_t)i];
+    const int k = (int)std::min<uint64_t>(s[i].top_k, (uint64_t)INT32_MAX);
+    in[(size_t)r] = u[i];
+    in[(size_t)(rows + r)] = s[i].temperature;
+    memcpy(&in[(size_t)(2 * rows + r)], &k, sizeof(int));
+    in[(size_t)(3 * rows + r)] = s[i].top_p;
+    in[(size_t)(4 * rows + r)] = min_p ? min_p[i] : 0.f;
+  }
+  IFX_CUDA(cudaMemcpyAsync(sample_buf, in.data(), in.size() * sizeof(float), cudaMemcpyHostToDevice, st));
+  float *b = sample_buf, *o = b + (size_t)5 * rows;
+  const int64_t V = (int64_t)cfg.vocab_size;
+  SampleRowsArgs a{of_model ? logits : kb->logits, rows, V, V, b, b + rows, reinterpret_cast<int *>(b + 2 * rows),
+                   b + 3 * rows, b + 4 * rows, reinterpret_cast<int *>(o), o + rows};
+  IFX_TRY(op_sample_rows(a, st));
+  IFX_CUDA(cudaMemcpyAsync(out.data(), o, out.size() * sizeof(float), cudaMemcpyDeviceToHost, st));
+  IFX_TRY(step_sync(st));
+  for (int i = 0; i < n; ++i) {
+    const int r = of_model ? 0 : kb->order[(size_t)i];
+    memcpy(&tokens[i], &out[(size_t)r], sizeof(uint32_t));
+    if (logprobs) logprobs[i] = out[(size_t)(rows + r)];
+  }
+  return IFX_OK;
 }
 
 ifx_status Model::step_sync(cudaStream_t st) {
@@ -1247,6 +1454,18 @@ ifx_status Model::tp_usable() const {
 ifx_status Model::reset_seq(KvBatch &kb, int seq) {
   if (seq < 0 || seq >= kb.batch) return fail(IFX_ERR_INVALID_ARGUMENT, "batch: no such sequence");
   IFX_CUDA(cudaSetDevice(device));
+  std::vector<int> done;
+  if (kb.q4) {
+    done.assign((size_t)kb.batch, 0);
+    done[(size_t)seq] = 1;
+    IFX_CUDA(cudaMemcpyAsync(kb.add4, done.data(), sizeof(int) * kb.batch, cudaMemcpyHostToDevice, stream));
+    int *nf = kb.lens4 + kb.batch;
+    PagesReleaseArgs r{kb.add4, kb.pos, kb.batch, kb.table_dev, kb.max_pages, kb.free4, (int)kb.n_pages, kb.n_free4, kb.lens4, nf};
+    IFX_TRY(op_pages_release(r, stream));
+    IFX_CUDA(cudaMemcpyAsync(kb.n_free4, nf, sizeof(int), cudaMemcpyDeviceToDevice, stream));
+    kb.n_free += (size_t)kb.held[(size_t)seq];
+    kb.held[(size_t)seq] = 0;
+  }
   IFX_CUDA(cudaMemsetAsync(kb.pos + seq, 0, sizeof(int), stream));
   IFX_CUDA(cudaStreamSynchronize(stream));
   kb.len[(size_t)seq] = 0;
@@ -1299,7 +1518,9 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
   }
   IFX_CUDA(cudaSetDevice(device));
   cudaStream_t st = stream;
+  if (kb.q4) IFX_TRY(kb.take(nullptr, kb.batch, n));
   for (int b = 0; b < kb.batch; ++b) IFX_TRY(kb.reserve(b, kb.len[(size_t)b] + n, st));
+  if (n) kb.latest_rows(kb.batch);
   uint32_t *toks = nullptr;  // every step's tokens, copied out once at the end
   IFX_TRY(dalloc(&toks, std::max<size_t>(1, n) * kb.batch));
   IFX_CUDA(cudaMemcpyAsync(kb.ids, tokens, sizeof(uint32_t) * kb.batch, cudaMemcpyHostToDevice, st));
@@ -1369,7 +1590,11 @@ ifx_status Model::run_prompt(KvCache *kvp, const uint32_t *ids, size_t n, float 
     IFX_TRY(op_rope(w_k, n, G, hd, c.rope_dim, c.rope_base, pos0, st));
     if (kvp) {
       KvCache &kv = *kvp;
-      if (kv.page_table)
+      if (kv.q4) {
+        Kv4RowsArgs r{w_k, w_v, nullptr, nullptr, IFX_TYPE_F32, N, kvd, kvd, kv.q4->slots4,
+                      kv.q4->pages4 + l * kv.q4->layer_bytes, (int64_t)kv.q4->n_pages, G, hd};
+        IFX_TRY(op_kv4_store(r, st));
+      } else if (kv.page_table)
         kv_write_paged_kernel<<<(unsigned)n, 256, 0, st>>>(w_k, w_v, kv.k + l * kv.per_layer,
                                                            kv.v + l * kv.per_layer, (int)n, G, hd,
                                                            kv.page_rows, kv.page_stride,
@@ -1381,7 +1606,7 @@ ifx_status Model::run_prompt(KvCache *kvp, const uint32_t *ids, size_t n, float 
       IFX_CUDA(cudaGetLastError());
     }
     PrefillAttnArgs pa{w_q, w_k, w_v, w_attn, (int)n, H, G, hd, kvp ? 1 : 0};
-    if (kvp) {  // the chunk's K/V rows were just written to the cache: stream them from there
+    if (kvp && !kvp->q4) {  // the chunk's K/V rows were just written to the cache: stream them from there
       const KvCache &kv = *kvp;
       pa.kc = kv.k + l * kv.per_layer;
       pa.vc = kv.v + l * kv.per_layer;

@@ -37,6 +37,9 @@ struct KvCache {  // KvCache (src/model/cache.rs:7-14), f16 on the device
   const int *page_table = nullptr;
   int page_rows = 0;
   int64_t page_stride = 0;
+  // a view of one sequence of a KvBatch in 4 bits: its rows go to the slots
+  // the batch has laid out (KvBatch::slots4)
+  struct KvBatch *q4 = nullptr;
   int dev = -1;                       // device of the allocations (the destructor must
                                       // not read the model: it may be freed first)
   ifx_status create(Model *model, size_t max_seq_len);
@@ -84,6 +87,32 @@ struct KvBatch {
   // captured after one eager step has run (first-call attribute setup)
   cudaGraphExec_t graph = nullptr;
   bool warm = false;
+  // 4-bit mode (no reference counterpart): the cache is a pool of pages in
+  // the layout of serve.cuh, layer l's at pages4 + l * layer_bytes, one table
+  // for all layers. Pages, slots and positions of a step's rows are built on
+  // the device (op_pages_extend / op_pages_release); the host only counts.
+  bool q4 = false;
+  uint8_t *pages4 = nullptr;
+  int64_t layer_bytes = 0;
+  int *free4 = nullptr, *n_free4 = nullptr;   // the free list and its length (device)
+  int *add4 = nullptr, *ones4 = nullptr;      // new rows of each sequence: a subset's, every one's
+  int *lens4 = nullptr;                       // lengths with the step's rows, then n_free', q_start, status
+  int *slots4 = nullptr, *positions4 = nullptr;
+  void *ws4 = nullptr;
+  size_t ws4_bytes = 0;
+  std::vector<int> held;                      // pages each sequence holds
+  size_t n_free = 0;
+  ifx_status create_q4(Model *model, size_t max_seq_len, int nseq, size_t pages);
+  ifx_status common(const ifx_config &c, int nseq);
+  // count the pages that `rows` more rows of each listed sequence need; fails
+  // with no change when there are too few
+  ifx_status take(const int *seqs, int n, size_t rows);
+  ifx_status extend(const int *add, size_t max_tokens, cudaStream_t st);
+  // the rows that sampling draws from: those of the latest step (caller's row
+  // i at order[i]), or the latest prompt's last one
+  std::vector<int> order;
+  bool after_prompt = false;
+  void latest_rows(int n);
   ifx_status create(Model *model, size_t max_seq_len, int nseq, size_t pages = 0);
   // give sequence `seq` pages for positions [0, rows); fails with no change
   // when the pool runs out
@@ -187,6 +216,10 @@ struct Model {
   ifx_status decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const uint32_t *tokens,
                                float *logits_host, uint32_t *argmax_host);
   ifx_status reset_seq(KvBatch &kb, int seq);
+  // draws for n rows of the batch's latest logits (kb null: the model's)
+  ifx_status sample_batch(KvBatch *kb, int n, const ifx_sampler *s, const float *min_p, const float *u,
+                          uint32_t *tokens, float *logprobs);
+  float *sample_buf = nullptr;  // settings and draws of at most kGemmSmallMax rows
   // the end of a call's device work: a bounded wait that aborts the
   // communicator under tensor parallelism (tp_wait), else a stream sync
   ifx_status step_sync(cudaStream_t st);

@@ -172,7 +172,7 @@ unsigned grid_for(int64_t items) {
 ifx_status op_pages_extend(const PagesExtendArgs &a, cudaStream_t st) {
   const size_t smem = (size_t)a.n_seqs * 3 * sizeof(int);
   static std::atomic<uint64_t> done{0};
-  if (smem > 48 * 1024) IFX_TRY(raise_smem(pages_extend_kernel, kMaxServeSeqs * 12, done));
+  IFX_TRY(raise_smem(pages_extend_kernel, kMaxServeSeqs * 12, done));
   pages_extend_kernel<<<grid_for(a.max_tokens), kPagesThreads, smem, st>>>(a);
   IFX_CUDA(cudaGetLastError());
   return IFX_OK;

@@ -830,7 +830,7 @@ template <bool IN_SMEM, int PER_SM>
 ifx_status run(const SampleRowsArgs &a, int cluster, size_t smem, cudaStream_t st) {
   auto kernel = sample_rows_kernel<IN_SMEM, PER_SM>;
   static std::atomic<uint64_t> done{0};
-  if (smem > 48 * 1024) IFX_TRY(raise_smem(kernel, 220 * 1024, done));
+  IFX_TRY(raise_smem(kernel, 216 * 1024, done));
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
@@ -853,7 +853,11 @@ ifx_status run(const SampleRowsArgs &a, int cluster, size_t smem, cudaStream_t s
     part.token = a.token + at;
     part.logprob = a.logprob ? a.logprob + at : nullptr;
     cfg.gridDim = dim3((unsigned)cluster, (unsigned)part.rows);
-    IFX_CUDA(cudaLaunchKernelEx(&cfg, kernel, part));
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, part);
+    if (e != cudaSuccess) {
+      cudaGetLastError();  // reported here, not to the next call
+      return cuda_fail(e, "sample_rows");
+    }
   }
   return IFX_OK;
 }

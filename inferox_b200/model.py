@@ -94,11 +94,13 @@ class Model:
     def kv_cache(self, max_seq: int | None = None) -> "KvCache":
         return KvCache(self, max_seq or int(self.config.context_length))
 
-    def kv_batch(self, batch: int, max_seq: int | None = None, pages: int = 0) -> "KvBatch":
+    def kv_batch(self, batch: int, max_seq: int | None = None, pages: int = 0, kv_bits: int = 16) -> "KvBatch":
         """`batch` independent sequences decoded together (one weight read per
         step). pages > 0: the caches share a pool of that many 64-position
-        pages, taken as sequences grow and returned by reset()."""
-        return KvBatch(self, batch, max_seq or int(self.config.context_length), pages)
+        pages, taken as sequences grow and returned by reset(). kv_bits=4: the
+        paged cache is held in 4 bits (Q4_0 rows); without `pages` the pool
+        holds every sequence at its longest."""
+        return KvBatch(self, batch, max_seq or int(self.config.context_length), pages, kv_bits)
 
     def prefill(self, ids, kv: "KvCache", last_row_only: bool = False) -> np.ndarray:
         ids = np.ascontiguousarray(ids, np.uint32)
@@ -188,10 +190,15 @@ class KvBatch:
 
     PAGE_ROWS = 64
 
-    def __init__(self, model: Model, batch: int, max_seq: int, pages: int = 0):
+    def __init__(self, model: Model, batch: int, max_seq: int, pages: int = 0, kv_bits: int = 16):
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, not {kv_bits!r}")
         self._model = model
         h = C.c_void_p()
-        if pages:
+        if kv_bits == 4:
+            pages = pages or batch * (-(-max_seq // self.PAGE_ROWS))
+            check(lib.ifx_kv_batch_create_q4(model._h, max_seq, batch, pages, C.byref(h)), "kv_batch_create_q4")
+        elif pages:
             check(lib.ifx_kv_batch_create_paged(model._h, max_seq, batch, pages, C.byref(h)),
                   "kv_batch_create_paged")
         else:
@@ -253,6 +260,12 @@ class KvBatch:
               "decode_step_batch_seqs")
         return (logits[: s.size * m.vocab].reshape(s.size, m.vocab) if want_logits else None), amax[: s.size]
 
+    def sample(self, samplers, u):
+        """Tokens for rows 0.. of the latest decode step (its own row order), or
+        for the latest prompt's last row: row i by samplers[i] and the uniform
+        draw u[i] in [0, 1), on the device. Returns (tokens, logprobs)."""
+        return _sample_batch(self._model, self._h, samplers, u)
+
     def reset(self, seq: int) -> None:
         """KvCache::clear of one sequence, so a new request can take its place."""
         check(lib.ifx_kv_batch_reset(self._model._h, self._h, seq), "kv_batch_reset")
@@ -268,13 +281,38 @@ class KvBatch:
         return out[: n_steps * self.batch].reshape(n_steps, self.batch), (float(ms.value) if timed else None)
 
 
+def uniform(seed: int, offset: int) -> float:
+    """The uniform draw of (seed, offset) that Sampler.sample uses: a counter
+    hashed to 23 bits."""
+    m = (1 << 64) - 1
+    z = (seed + 0x9E3779B97F4A7C15 * (offset + 1)) & m
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & m
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & m
+    return ((z ^ (z >> 31)) >> 41) / 8388608.0
+
+
+def _sample_batch(model: "Model", kb, samplers, u):
+    n = len(samplers)
+    if n != len(u):
+        raise ValueError("one draw per sampler")
+    s = (SamplerC * max(n, 1))(*(x._c() for x in samplers))
+    mp = np.ascontiguousarray([x.min_p for x in samplers], np.float32)
+    draws = np.ascontiguousarray(u, np.float32)
+    tok, logp = np.empty(max(n, 1), np.uint32), np.empty(max(n, 1), np.float32)
+    check(lib.ifx_sample_batch(model._h, kb, n, s, _f32(mp), _f32(draws), _u32(tok), _f32(logp)), "sample_batch")
+    return tok[:n], logp[:n]
+
+
 @dataclass
 class Sampler:
-    """Sampler (src/sampler.rs:8-16); sampling runs on the device."""
+    """Sampler (src/sampler.rs:8-16); sampling runs on the device. min_p (no
+    reference counterpart) keeps tokens of at least that share of the most
+    likely one's probability."""
 
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
+    min_p: float = 0.0
 
     @classmethod
     def greedy(cls) -> "Sampler":
@@ -285,10 +323,12 @@ class Sampler:
 
     def sample(self, model: Model, seed: int = 0, offset: int = 0) -> int:
         """Sample from the model's latest logits (prefill or decode_step)."""
+        if self.min_p > 0:
+            return int(_sample_batch(model, None, [self], [uniform(seed, offset)])[0][0])
         out = C.c_uint32()
         s = self._c()
         check(lib.ifx_sample(model._h, C.byref(s), seed, offset, C.byref(out)), "Sampler::sample")
         return int(out.value)
 
 
-__all__ = ["Model", "KvCache", "KvBatch", "Sampler", "IfxError", "load_opts"]
+__all__ = ["Model", "KvCache", "KvBatch", "Sampler", "IfxError", "load_opts", "uniform"]

@@ -9,6 +9,11 @@ maxima, forward.rs:615-622), then the argmax after feeding each token back.
     rid = srv.submit(prompt_ids, max_tokens=64)
     results = srv.run()            # {request id: generated tokens}
 
+A request submitted with a `sampler` (and a `seed`) draws its tokens instead:
+token i is drawn from its row's logits with the uniform number of (seed, i),
+as Sampler.sample(model, seed, i) draws it, on the device for all rows of a
+step at once. Greedy requests beside it keep their results.
+
 Each step() first admits waiting requests into free slots (first come,
 first served: the slot is cleared, the prompt prefilled, its first token
 taken), then runs one decode step of every active slot together
@@ -19,7 +24,7 @@ not fed back (the reference feeds it and discards the logits), so a request
 needs len(prompt) + max_tokens - 1 cache rows.
 
 Over a paged batch (Server.for_model(..., pages=P): the slots share a pool
-of P cache pages) the pool can run dry. A prefill that finds too few pages
+of P cache pages; kv_bits=4 holds it in 4 bits) the pool can run dry. A prefill that finds too few pages
 leaves its request waiting at the front until a finishing request returns
 some; a decode step that finds none preempts the most recently admitted
 request (its slot is reset, returning its pages, and it starts again from
@@ -32,6 +37,8 @@ from collections import deque
 from dataclasses import dataclass, field
 
 import numpy as np
+
+from .model import Sampler, uniform
 
 
 def _pool_empty(e: BaseException) -> bool:
@@ -51,6 +58,8 @@ class _Request:
     prompt: np.ndarray
     max_tokens: int
     eos: int | None
+    sampler: object = None  # None: greedy
+    seed: int = 0
     tokens: list = field(default_factory=list)
     done: bool = False
     order: int = 0  # admission count when it took its slot
@@ -58,8 +67,9 @@ class _Request:
 
 
 class Server:
-    """Greedy continuous batching over `batch`, any object with KvBatch's
-    `batch`, `max_seq`, `prefill`, `decode_step_seqs` and `reset`."""
+    """Continuous batching over `batch`, any object with KvBatch's `batch`,
+    `max_seq`, `prefill`, `decode_step_seqs` and `reset` (and `sample`, for
+    requests with a sampler)."""
 
     def __init__(self, batch):
         self.kb = batch
@@ -75,10 +85,10 @@ class Server:
         self.paged = bool(getattr(batch, "pages", None)) and batch.pages()[1] > 0
 
     @classmethod
-    def for_model(cls, model, slots: int, max_seq: int, pages: int = 0) -> "Server":
-        return cls(model.kv_batch(slots, max_seq, pages))
+    def for_model(cls, model, slots: int, max_seq: int, pages: int = 0, kv_bits: int = 16) -> "Server":
+        return cls(model.kv_batch(slots, max_seq, pages, kv_bits))
 
-    def submit(self, prompt, max_tokens: int, eos: int | None = None) -> int:
+    def submit(self, prompt, max_tokens: int, eos: int | None = None, sampler=None, seed: int = 0) -> int:
         p = np.ascontiguousarray(prompt, np.uint32)
         if p.size == 0:
             raise ValueError("empty prompt")
@@ -87,7 +97,7 @@ class Server:
         if p.size + max_tokens - 1 > self.kb.max_seq:
             raise ValueError(f"prompt ({p.size}) + max_tokens ({max_tokens}) - 1 exceeds the "
                              f"{self.kb.max_seq}-row cache of a slot")
-        r = _Request(self._next, p, max_tokens, eos)
+        r = _Request(self._next, p, max_tokens, eos, sampler, seed)
         self._next += 1
         self.requests[r.rid] = r
         self.waiting.append(r)
@@ -124,6 +134,7 @@ class Server:
                     self.kb.reset(slot)
                 self.used[slot] = True
                 logits = self.kb.prefill(slot, r.prompt, True)
+                first = last_argmax(logits[0]) if r.sampler is None else self._draw([r])[0]
             except BaseException as e:
                 # the request is not lost: it waits at the front again (the
                 # slot is reset before its next use)
@@ -131,11 +142,18 @@ class Server:
                 if _pool_empty(e) and self._active():
                     return  # pages come back when an active request finishes
                 raise
-            r.tokens.append(last_argmax(logits[0]))
+            r.tokens.append(first)
             r.order = self._admitted
             self._admitted += 1
             self.slots[slot] = r
             self._finish_if_done(slot)
+
+    def _draw(self, requests) -> list[int]:
+        """The next token of every request, row i of the latest logits its."""
+        greedy = Sampler.greedy()
+        toks, _ = self.kb.sample([r.sampler or greedy for r in requests],
+                                 [uniform(r.seed, len(r.tokens)) if r.sampler else 0.0 for r in requests])
+        return [int(t) for t in toks]
 
     def _preempt(self, seqs: list[int]) -> None:
         """Return the pages of the most recently admitted of `seqs`; its
@@ -166,6 +184,10 @@ class Server:
                     raise
                 self._preempt(seqs)
         self.steps += 1
+        rows = [self.slots[i] for i in seqs]
+        if any(r.sampler is not None for r in rows):
+            drawn = self._draw(rows)
+            amax = [a if r.sampler is None else d for r, a, d in zip(rows, amax, drawn)]
         for i, t in zip(seqs, amax):
             self.slots[i].tokens.append(int(t))
             self._finish_if_done(i)

@@ -158,6 +158,69 @@ def test_attention_chunks(hd, dtype):
     check_attention([100, 333, 64], [100, 70, 64], 8, 2, hd, dtype)
 
 
+@pytest.mark.parametrize("H,G,hd", [(4, 4, 64), (16, 4, 128), (8, 4, 32), (8, 4, 96), (4, 4, 256), (4, 4, 160)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_chunks_of_many_sequences(H, G, hd, window):
+    """Enough query rows for the kernel that takes 64 of them at a time."""
+    per = {64: 70, 128: 20, 32: 40, 96: 40, 256: 66, 160: 66}[hd]
+    qlens = [per] * 14 + [1, 0, per + 30, 3]
+    lens = [q + 37 * i % 150 for i, q in enumerate(qlens)]
+    lens[3], qlens[3] = per - 9, per  # rows before the cache's first
+    lens[15] = 0
+    check_attention(lens, qlens, H, G, hd, torch.float16 if hd == 32 else torch.float32, window=window)
+
+
+def test_attention_chunks_gaps_and_magnitudes():
+    """The same kernel: a missing page, rows behind the last sequence, a query
+    that is not finite, queries and values of very different sizes, a scale
+    below 0."""
+    H, G, hd, n, ql = 8, 8, 64, 20, 64
+    lens = [64 + 7 * i for i in range(n)]
+    rng = np.random.default_rng(6)
+    pages, table, K, V = filled(rng, lens, G, hd)
+    for b in range(0, n, 3):  # values from 1e-3 to 1e3 by sequence and by row
+        v = (10.0 ** rng.uniform(-3, 3) * rng.standard_normal((lens[b], G, hd)) *
+             10.0 ** rng.uniform(-1, 0, (lens[b], 1, 1))).astype(np.float32)
+        k = rng.standard_normal((lens[b], G, hd)).astype(np.float32)
+        t = np.arange(lens[b])
+        ops.kv4_store(cuda(k), cuda(v), i32(table[b, t // 64] * 64 + t % 64), pages)
+        K[b], V[b] = SR.values(*SR.quantise(k)), SR.values(*SR.quantise(v))
+    start = np.arange(n + 1) * ql
+    q = rng.standard_normal((n * ql + 5, H, hd)).astype(np.float32) * 10.0 ** rng.uniform(-2, 1, (n * ql + 5, 1, 1)).astype(np.float32)
+    table[1, 1] = -1  # rows 64 .. of sequence 1 are hidden: every row sees the first page
+    out = torch.full((n * ql + 5, H, hd), 7.0, device=DEV)
+    got = ops.kv4_attention(cuda(q), pages, i32(table), i32(lens), G, q_start=i32(start), scale=-0.11, out=out).cpu().numpy()
+    assert (got[n * ql:] == 7).all()
+    for b in range(n):
+        sl = slice(start[b], start[b + 1])
+        if b == 1:
+            k, v, rows = K[1][:64], V[1][:64], q[sl]
+            ref = np.zeros((ql, H, hd))
+            for i in range(ql):
+                e = lens[1] - ql + i + 1
+                r, worst = SR.attention(rows[i:i + 1], [k[:min(e, 64)]], [v[:min(e, 64)]], [min(e, 64)], [0, 1], -0.11)
+                ref[i] = r[0]
+        else:
+            k, v = K[b], V[b]
+            ref, worst = SR.attention(q[sl], [k], [v], [lens[b]], [0, ql], -0.11)
+        lim = bound(ref, [k], [v], worst, torch.float32)
+        assert np.all(np.abs(got[sl] - ref) <= lim), (b, float((np.abs(got[sl] - ref) / lim).max()))
+    bad = cuda(q)
+    bad[70, 3, 5] = np.nan
+    bad[71, 2, 5] = np.inf
+    got = ops.kv4_attention(bad, pages, i32(table), i32(lens), G, q_start=i32(start), scale=-0.11)
+    nan = torch.isnan(got).all(-1)
+    assert nan[70, 3] and nan[71, 2] and nan.sum() == 2 and torch.isnan(got).sum() == 2 * hd
+
+
+def test_attention_query_that_is_not_finite():
+    pages, table, _, _ = filled(np.random.default_rng(1), [90, 200], 2, 64)
+    q = torch.randn(2, 8, 64, device=DEV)
+    q[0, 3, 7], q[1, 5, 0] = np.nan, -np.inf
+    got = torch.isnan(ops.kv4_attention(q, pages, i32(table), i32([90, 200]), 2))
+    assert got[0, 3].all() and got[1, 5].all() and got.sum() == 2 * 64
+
+
 def test_attention_empty_rows_and_gaps():
     """kv_len 0, query rows before the cache's first row, sequences without
     query rows, rows behind the last sequence, and a table entry of -1."""
@@ -310,7 +373,8 @@ def test_extend_edges():
     assert check_extend([256], [1], 4, 3, 1) == 2
     assert check_extend([255], [1], 4, 0, 1) == 0
     assert check_extend([0, 64, 128], [200000, 1, 0], 4000, 3200, 200001) == 0
-    assert check_extend([3] * 8192, [1] * 8192, 1, 0, 8192) == 0
+    for n in (4096, 8192):
+        assert check_extend([3] * n, [1] * n, 1, 0, n) == 0
 
 
 @pytest.mark.parametrize("n", [1, 40, 700])
@@ -360,7 +424,7 @@ def check_sample(z, u, t, k, p, m):
     return token
 
 
-@pytest.mark.parametrize("n", [1, 2, 31, 1000, 4097, 32000, 128256, 300001])
+@pytest.mark.parametrize("n", [1, 2, 31, 1000, 2048, 2300, 4097, 32000, 128256, 300001])
 def test_sample_settings(n):
     rng = np.random.default_rng(n)
     rows = 40 if n <= 32000 else 12

@@ -205,3 +205,42 @@ def test_paged_pool_too_small_for_one_request():
     srv2.submit([3, 4, 5], 12)  # fits at admission, outgrows the pool alone
     with pytest.raises(PoolEmpty):
         srv2.run()
+
+
+class SampledFake(FakeBatch):
+    """Its `sample` hashes the row's history with the draw, so a token depends
+    on nothing but the request's own history, sampler and seed."""
+
+    def prefill(self, slot, ids, last_row_only=False):
+        self.rows = [slot]
+        return super().prefill(slot, ids, last_row_only)
+
+    def decode_step_seqs(self, seqs, tokens, want_logits=True):
+        self.rows = list(seqs)
+        return super().decode_step_seqs(seqs, tokens, want_logits)
+
+    def sample(self, samplers, u):
+        assert len(samplers) == len(u) == len(self.rows)
+        toks = [(_next(self.hist[s]) + (int(x * 8388608) % 13 if p.temperature > 0 else 0)) % V
+                for s, p, x in zip(self.rows, samplers, u)]
+        return np.array(toks, np.uint32), np.zeros(len(toks), np.float32)
+
+
+def test_sampled_requests_do_not_depend_on_their_neighbours():
+    from inferox_b200 import Sampler
+    from inferox_b200.model import uniform
+    rng = np.random.default_rng(3)
+    reqs = [(rng.integers(0, V, 3 + i).tolist(), 5 + 2 * i, Sampler(0.9, 5) if i % 3 else None, 40 + i) for i in range(8)]
+    alone = []
+    for p, k, s, seed in reqs:
+        srv = Server(SampledFake(1, 100))
+        rid = srv.submit(p, k, sampler=s, seed=seed)
+        alone.append(srv.run()[rid])
+    srv = Server(SampledFake(3, 100))
+    rids = [srv.submit(p, k, sampler=s, seed=seed) for p, k, s, seed in reqs]
+    got = srv.run()
+    assert [got[r] for r in rids] == alone
+    # a greedy request beside sampled ones is _alone()'s
+    assert alone[0] == _alone(reqs[0][0], reqs[0][1])
+    assert 0 <= min(uniform(s, o) for s in range(50) for o in range(50)) and max(
+        uniform(s, o) for s in range(50) for o in range(50)) < 1
