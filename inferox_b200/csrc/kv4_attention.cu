@@ -124,18 +124,15 @@ __device__ __forceinline__ void mma_su(int (&d)[4], const uint32_t (&a)[4], uint
 
 constexpr uint32_t kHigh = 0xf0f0f0f0u, kSign = 0x80808080u;
 
-// x + kMagic, |x| <= kTop, has the bits kMagicBits + rint(x): byte 0 and byte
+// x + kMagic, |x| <= kTop, has the bits 0x4b400000 + rint(x): byte 0 and byte
 // 1 are the integer's low digits (unsigned, to base 256), byte 2 is 64 + its
-// signed top digit. As the start of an s32 accumulator kMagicBits makes the
-// sum's bits those of the float kMagic + sum while |sum| < 2^22.
+// signed top digit.
 constexpr float kMagic = 12582912.f;
-constexpr int kMagicBits = 0x4b400000;
 constexpr float kTop = 4.1e6f;
 
-// 65536 top + 256 mid + low of the three planes' sums: top comes doubled,
-// low as kMagic + low.
+// 65536 top + 256 mid + low of the three planes' sums; top comes doubled.
 __device__ __forceinline__ float planes(int top2, int mid, int low) {
-  return fmaf((float)((top2 << 7) + mid), 256.f, __int_as_float(low) - kMagic);
+  return fmaf((float)((top2 << 7) + mid), 256.f, (float)low);
 }
 
 __device__ __forceinline__ float quad_rows_sum(float v) {  // over the lanes of one column pair
@@ -251,11 +248,17 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
   constexpr int PAIRS = L::kPairs, HD = L::kHd, TT = (NT + 1) / 2, TB = Kv4Layout::tile_bytes(NB), HB = L::kHalf;
   constexpr int SC = 256 * NB;  // the scales behind a half tile's words
   extern __shared__ __align__(128) uint8_t sm[];
-  uint64_t *bar = reinterpret_cast<uint64_t *>(sm + L::kBars) + (threadIdx.x >> 5) * 2;
   long long *pre = reinterpret_cast<long long *>(sm + L::kBytes);  // [n_seqs + 1]
   __shared__ long long s_scan[NW];
+  // what a warp needs between segments only: kept out of its registers
+  __shared__ Segment s_now[NW];
+  __shared__ int s_next[NW];  // the sequence of the copies
+  __shared__ long long s_range[NW][2], s_cta[2];  // units of the warp, of the CTA
   __shared__ int s_seq[2 * NW][3], s_whole[2 * NW], s_join[2 * NW];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  // the warp index by shuffle: the compiler keeps what follows from it in
+  // uniform registers
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint64_t *bar = reinterpret_cast<uint64_t *>(sm + L::kBars) + warp * 2;
   if (lane == 0) {
     mbar_init(&bar[0], 1);
     mbar_init(&bar[1], 1);
@@ -284,8 +287,6 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
     for (int i = 0; i < warp; ++i) base += s_scan[i];
     for (int b = b0; b < b1; ++b) pre[b] += base;
     if (tid == NW * 32 - 1) pre[n] = base + mine;
-    __syncthreads();
-  } else {
     __syncthreads();
   }
   const int grp = a.H / a.G;
@@ -317,17 +318,26 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
       info[blockIdx.x] = RangeInfo{s.begin, s.end, total, s.seq, s.h, s.ct, live};
     }
   }
+  if (tid == 0) s_cta[0] = c0, s_cta[1] = c1;
+  __syncthreads();
   const int share = (int)(c1 - c0);
   const long long u0 = c0 + (int64_t)share * warp / NW, u1 = c0 + (int64_t)share * (warp + 1) / NW;
 
   // ---- the warp's pages
   if (u0 < u1) {
     if (!a.alone) s = locate<PAIRS>(a, pre, u0);
+    if (lane == 0) {
+      s_now[warp] = s;
+      s_next[warp] = s.seq;
+      s_range[warp][0] = u0;
+      s_range[warp][1] = u1;
+    }
+    __syncwarp();
     uint8_t *kbuf = sm + warp * L::kPage, *vbuf = kbuf + 4 * HB;
     // cursor of the copies, one page ahead
-    int fseq = s.seq, fh = s.h, flen = s.len, fj = s.lo + (int)(u0 - s.begin), frem = (int)(s.end - u0), fleft = (int)(u1 - u0);
-    auto page_at = [&]() { return fj < a.max_pages ? __ldg(a.table + (size_t)fseq * a.max_pages + fj) : -1; };
-    int fpage = fleft > 0 ? page_at() : -1;
+    int fj = s.lo + (int)(u0 - s.begin), frem = (int)(s.end - u0), fleft = (int)(u1 - u0), fh = s.h, flen = s.len;
+    auto page_at = [&]() { return fj < a.max_pages ? __ldg(a.table + (size_t)s_next[warp] * a.max_pages + fj) : -1; };
+    int fpage = page_at();
     auto copy = [&](int half, bool more) {  // keys (0) or values (1) of the page at the cursor
       if (!more) return;
       const bool ok = (unsigned)fpage < (unsigned)a.n_pages;
@@ -347,7 +357,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
 
     int left = (int)(u1 - u0);
     uint32_t phase = 0;
-    const int czero[4] = {0, 0, 0, 0}, cmagic[4] = {0, kMagicBits, 0, kMagicBits};
+    const int czero[4] = {0, 0, 0, 0};
     while (left > 0) {
       // ---- query columns of this segment: lane (g, t) holds column g, that
       // is plane 1 (g even) or 0 (g odd) of pair g >> 1, at dimensions 8 t ..
@@ -355,6 +365,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
       uint32_t q[NT][NB][2], qt[TT][NB][2];
       int jmax[NT], jmin[NT];
       float qscale[NT];
+      const Segment &s = s_now[warp];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         int head;
@@ -436,8 +447,10 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
           for (int i = 0; i < 4; ++i) o[nt][b][i] = 0.f;
       }
 
-      int row0 = (s.lo + (int)(u1 - left - s.begin)) * kKv4PageRows;
-      int todo = min(left, (int)(s.end - (u1 - left)));
+      const int len = s.len;
+      const long long at = s_range[warp][1] - left;
+      int row0 = (s.lo + (int)(at - s.begin)) * kKv4PageRows;
+      int todo = min(left, (int)(s.end - at));
       left -= todo;
       for (; todo > 0; --todo, row0 += kKv4PageRows) {
         // the cursor moves to the next page (its table entry is on its way
@@ -449,14 +462,17 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
         const bool more = fleft > 0;
         if (more) {
           if (frem == 0) {
-            const Segment n = locate<PAIRS>(a, pre, u1 - fleft);
-            fseq = n.seq, fh = n.h, flen = n.len, fj = n.lo, frem = (int)(n.end - n.begin);
+            const Segment n = locate<PAIRS>(a, pre, s_range[warp][1] - fleft);
+            fj = n.lo, frem = (int)(n.end - n.begin), fh = n.h, flen = n.len;
+            __syncwarp();
+            if (lane == 0) s_next[warp] = n.seq;
+            __syncwarp();
           }
           fpage = page_at();
         }
         // rows that hold nothing (behind the last one, or of a page that does
         // not exist) get scale 0, whatever bytes are there
-        const int live_rows = here ? s.len - row0 : 0;
+        const int live_rows = here ? len - row0 : 0;
         const bool clear = live_rows < kKv4PageRows;
         auto wipe = [&](uint8_t *buf) {
           for (int r = max(0, live_rows) + lane; r < kKv4PageRows; r += 32)
@@ -490,7 +506,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               int acc[4];
-              mma_su(acc, w, q[nt][b][0], q[nt][b][1], cmagic);
+              mma_su(acc, w, q[nt][b][0], q[nt][b][1], czero);
               sc[i][nt][0] = fmaf(d0[b], planes(top[nt / 2][nt & 1], acc[0], acc[1]), sc[i][nt][0]);
               sc[i][nt][1] = fmaf(d1[b], planes(top[nt / 2][2 + (nt & 1)], acc[2], acc[3]), sc[i][nt][1]);
             }
@@ -620,7 +636,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 if (i) mma_su(acc[nt], w, lo[nt][i], lo[nt][i + 1], acc[nt]);
-                else mma_su(acc[nt], w, lo[nt][i], lo[nt][i + 1], cmagic);
+                else mma_su(acc[nt], w, lo[nt][i], lo[nt][i + 1], czero);
               }
             }
 #pragma unroll
@@ -638,8 +654,9 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
       }
 
       // ---- the segment's end, or the range's
-      const bool whole = s.begin >= u0 && s.end <= u1;
-      const int slot = 2 * warp + (s.begin > u0 || s.end <= u0 ? 1 : 0);
+      const long long from = s_range[warp][0], to = s_range[warp][1];
+      const bool whole = s.begin >= from && s.end <= to;
+      const int slot = 2 * warp + (s.begin > from ? 1 : 0);
       float *part = L::part(sm, slot);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -664,10 +681,15 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
         s_seq[slot][0] = s.seq;
         s_seq[slot][1] = s.h;
         s_seq[slot][2] = s.ct;
-        s_whole[slot] = s.begin >= c0 && s.end <= c1;
-        s_join[slot] = s.begin <= c0 ? 0 : 1;
+        s_whole[slot] = s.begin >= s_cta[0] && s.end <= s_cta[1];
+        s_join[slot] = s.begin <= s_cta[0] ? 0 : 1;
       }
-      if (left > 0) s = locate<PAIRS>(a, pre, u1 - left);
+      if (left > 0) {
+        const Segment n = locate<PAIRS>(a, pre, to - left);
+        __syncwarp();
+        if (lane == 0) s_now[warp] = n;
+        __syncwarp();
+      }
     }
   }
   __syncthreads();
@@ -1312,7 +1334,7 @@ ifx_status run_nb(const Kv4AttnArgs &a, cudaStream_t st) {
     return !a.q_start && (int64_t)a.n_seqs * a.G * ((a.H / a.G + pairs - 1) / pairs) <= kNumSMs && a.max_pages <= 4 * warps;
   };
   if constexpr (NB <= 4) {
-    if (columns > 4) return run<NB, 2, 8, 1>(a, alone(8, 8), st);
+    if (columns > 4) return run<NB, 2, 12, 1>(a, alone(8, 12), st);
     if (alone(4, 12)) return run<NB, 1, 12, 1>(a, true, st);
     return run<NB, 1, 6, 2>(a, false, st);
   } else {
