@@ -74,11 +74,6 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], uint16_t &scale) {
   return w;
 }
 
-struct RowItem {
-  int64_t row;
-  int slot, h, b, t;  // destination row, kv head, block, lane of the block's four
-};
-
 // Where (slot, head) lives: its tile, and the row within it.
 __device__ __forceinline__ int64_t tile_offset(int slot, int h, int G, int nb) {
   return ((int64_t)(slot / kKv4PageRows) * G + h) * Kv4Layout::head_bytes(nb) +
@@ -91,11 +86,11 @@ __device__ __forceinline__ int64_t tile_offset(int slot, int h, int G, int nb) {
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) kv4_store_kernel(const __grid_constant__ Kv4RowsArgs a) {
   const int nb = a.hd / 32, lanes = a.G * nb * 4;  // threads per row
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const int64_t row = i / lanes;
+  const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;  // below 2^31: the launch sees to it
+  const int64_t row = i / (uint32_t)lanes;
   // whole groups of four lanes share a row and a block; lanes beyond the
   // rows keep running for the shuffles
-  const int e = (int)(i - row * lanes), h = e / (nb * 4), b = e / 4 % nb, t = e % 4;
+  const uint32_t e = i - (uint32_t)row * lanes, h = e / (uint32_t)(nb * 4), b = e / 4 % (uint32_t)nb, t = e % 4;
   int slot = -1;
   if (row < a.n) slot = a.slots[row];
   if (slot < 0 || slot / kKv4PageRows >= a.n_pages) slot = -1;
@@ -123,10 +118,10 @@ __global__ void __launch_bounds__(kRowThreads) kv4_store_kernel(const __grid_con
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(const __grid_constant__ Kv4RowsArgs a) {
   const int nb = a.hd / 32, lanes = a.G * nb * 4;
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const int64_t row = i / lanes;
+  const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;
+  const int64_t row = i / (uint32_t)lanes;
   if (row >= a.n) return;
-  const int e = (int)(i - row * lanes), h = e / (nb * 4), b = e / 4 % nb, t = e % 4;
+  const uint32_t e = i - (uint32_t)row * lanes, h = e / (uint32_t)(nb * 4), b = e / 4 % (uint32_t)nb, t = e % 4;
   const int slot = a.slots[row];
   float x[8] = {}, y[8] = {};
   if (slot >= 0 && slot / kKv4PageRows < a.n_pages) {
@@ -149,31 +144,37 @@ __global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(const __grid_cons
   store8(static_cast<T *>(a.v_out) + at, y);
 }
 
-unsigned row_blocks(const Kv4RowsArgs &a) {
-  const int64_t items = a.n * a.G * (a.hd / 32) * 4;
-  return (unsigned)((items + kRowThreads - 1) / kRowThreads);
+// One launch per 2^31 - kRowThreads threads or less.
+template <typename F>
+ifx_status in_parts(const Kv4RowsArgs &all, F launch) {
+  const int64_t lanes = (int64_t)all.G * (all.hd / 32) * 4, most = ((int64_t)INT32_MAX - kRowThreads) / lanes;
+  const int64_t size = all.type == IFX_TYPE_F16 ? 2 : 4, out = (int64_t)all.G * all.hd * size;
+  for (int64_t at = 0; at < all.n; at += most) {
+    Kv4RowsArgs a = all;
+    a.n = std::min(most, all.n - at);
+    a.slots += at;
+    if (a.k) a.k = static_cast<const char *>(a.k) + at * a.k_stride * size, a.v = static_cast<const char *>(a.v) + at * a.v_stride * size;
+    if (a.k_out) a.k_out = static_cast<char *>(a.k_out) + at * out, a.v_out = static_cast<char *>(a.v_out) + at * out;
+    launch((unsigned)((a.n * lanes + kRowThreads - 1) / kRowThreads), a);
+    IFX_CUDA(cudaGetLastError());
+  }
+  return IFX_OK;
 }
 
 }  // namespace
 
 ifx_status op_kv4_store(const Kv4RowsArgs &a, cudaStream_t st) {
-  if (!a.n) return IFX_OK;
-  if (a.type == IFX_TYPE_F16)
-    kv4_store_kernel<__half><<<row_blocks(a), kRowThreads, 0, st>>>(a);
-  else
-    kv4_store_kernel<float><<<row_blocks(a), kRowThreads, 0, st>>>(a);
-  IFX_CUDA(cudaGetLastError());
-  return IFX_OK;
+  return in_parts(a, [&](unsigned grid, const Kv4RowsArgs &p) {
+    if (p.type == IFX_TYPE_F16) kv4_store_kernel<__half><<<grid, kRowThreads, 0, st>>>(p);
+    else kv4_store_kernel<float><<<grid, kRowThreads, 0, st>>>(p);
+  });
 }
 
 ifx_status op_kv4_load(const Kv4RowsArgs &a, cudaStream_t st) {
-  if (!a.n) return IFX_OK;
-  if (a.type == IFX_TYPE_F16)
-    kv4_load_kernel<__half><<<row_blocks(a), kRowThreads, 0, st>>>(a);
-  else
-    kv4_load_kernel<float><<<row_blocks(a), kRowThreads, 0, st>>>(a);
-  IFX_CUDA(cudaGetLastError());
-  return IFX_OK;
+  return in_parts(a, [&](unsigned grid, const Kv4RowsArgs &p) {
+    if (p.type == IFX_TYPE_F16) kv4_load_kernel<__half><<<grid, kRowThreads, 0, st>>>(p);
+    else kv4_load_kernel<float><<<grid, kRowThreads, 0, st>>>(p);
+  });
 }
 
 }  // namespace ifx
