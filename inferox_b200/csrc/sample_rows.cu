@@ -114,15 +114,14 @@ struct Shared {
   Book book;
   double pow2[32];
   u64 red[kThreads / 32];
-  u64 best;            // this CTA's largest value and its last index
+  u64 best;            // this CTA's largest value (ordered bits)
   u64 mass;            // this CTA's mass: of all its tokens, or before the window
   u64 window[kWindow]; // ... and of each bucket in it
   u64 parts[kThreads / 32][kWindow];  // the same by warp
   u64 pick;
   int count, listed;   // tokens with w >= min_p; length of the list
   int place;
-  float zmax;
-  int last;
+  int last;            // greedy rows: the last index of the largest value
   // the leader's orders to the cluster
   int cmd, level, b0, lo, hi, masses, first;
 };
@@ -562,20 +561,33 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   int *hcount = reinterpret_cast<int *>(guess + kBuckets);        // [kBuckets]
   float *zs = reinterpret_cast<float *>(hcount + kBuckets);       // [per]
   auto value = [&](int i) { return IN_SMEM ? zs[i] : clean(zrow[lo + i]); };
+  auto four = [&](int i) {  // values i .. i + 3 (i a multiple of 4), NaN behind the last
+    float4 v;
+    if (IN_SMEM) {
+      v = *reinterpret_cast<const float4 *>(zs + i);
+    } else {
+      v.x = value(i);
+      v.y = i + 1 < len ? value(i + 1) : 0.f;
+      v.z = i + 2 < len ? value(i + 2) : 0.f;
+      v.w = i + 3 < len ? value(i + 3) : 0.f;
+    }
+    const float none = __uint_as_float(0x7fc00000u);
+    if (i + 4 > len) {
+      if (i + 1 >= len) v.y = none;
+      if (i + 2 >= len) v.z = none;
+      if (i + 3 >= len) v.w = none;
+    }
+    return v;
+  };
 
   const float T = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f;
   const float min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f, u_row = a.u[row];
   const int top_k = a.top_k ? a.top_k[row] : 0;
   if (tid < 32) sh.pow2[tid] = kPow2[tid];
-  // ---- read the row; its largest value and the last index that has it
+  if (tid == 0) sh.best = 0;
+  __syncthreads();
+  // ---- read the row; its largest value
   float top = -INFINITY;
-  int at = -1;
-  auto see = [&](float z, int i) {
-    if (z >= top) {
-      top = z;
-      at = i;
-    }
-  };
   if ((reinterpret_cast<uintptr_t>(zrow) & 15) == 0) {
     const float4 *src = reinterpret_cast<const float4 *>(zrow + lo);
 #pragma unroll 4
@@ -583,55 +595,28 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
       float4 v = __ldcs(src + i);
       v = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
       if (IN_SMEM) reinterpret_cast<float4 *>(zs)[i] = v;
-      see(v.x, 4 * i), see(v.y, 4 * i + 1), see(v.z, 4 * i + 2), see(v.w, 4 * i + 3);
+      top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
     for (int i = (len & ~3) + tid; i < len; i += kThreads) {
       const float z = clean(zrow[lo + i]);
       if (IN_SMEM) zs[i] = z;
-      see(z, i);
+      top = fmaxf(top, z);
     }
   } else {
     for (int i = tid; i < len; i += kThreads) {
       const float z = clean(zrow[lo + i]);
       if (IN_SMEM) zs[i] = z;
-      see(z, i);
+      top = fmaxf(top, z);
     }
   }
-  u64 best = at < 0 ? 0 : (u64)ordered(top) << 32 | (uint32_t)(lo + at);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) sh.red[warp] = best;
+  const uint32_t mine = __reduce_max_sync(0xffffffffu, ordered(top));
+  if (lane == 0) atomicMax(&sh.best, (u64)mine);
   for (int i = tid; i < kBuckets; i += kThreads) hcount[i] = 0;
-  __syncthreads();
   if (tid == 0) {
-    for (int i = 0; i < kThreads / 32; ++i) best = max(best, sh.red[i]);
-    sh.best = best;
     sh.count = 0;
     sh.listed = 0;
   }
-  cluster.sync();
-  if (warp == 0) {
-    best = lane < C ? cluster.map_shared_rank(&sh, lane)->best : 0;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) {
-      sh.last = (int)(uint32_t)best;
-      sh.zmax = unordered((uint32_t)(best >> 32));
-    }
-  }
-  __syncthreads();
   Row r;
-  r.zmax = sh.zmax;
-  const int last = sh.last;
-  const bool none = r.zmax == -INFINITY;
-  if (none || !(T > 0.f)) {
-    if (rank == 0 && tid == 0) {
-      a.token[row] = none ? -1 : last;
-      if (a.logprob) a.logprob[row] = none ? -INFINITY : 0.f;
-    }
-    cluster.sync();  // others may still read this CTA's maximum
-    return;
-  }
   r.s = min(50, 62 - (32 - __clz(n)));
   r.unit = __hiloint2double((1023 + r.s) << 20, 0);
   r.c = fmax(46.166241308446828 / (double)T, 1e-300);  // 32 log2(e) / T
@@ -640,16 +625,41 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   r.cut = (r.s + 2) * 0.6931471805599453 * (double)T;
   const float scale = (float)(kBuckets - 1) / (float)r.cut;
   const double u = fmin(fmax((double)u_row, 0.0), 1.0);
+  cluster.sync();
+  r.zmax = unordered(__reduce_max_sync(0xffffffffu, lane < C ? (uint32_t)cluster.map_shared_rank(&sh, lane)->best : 0u));
+  const bool none = r.zmax == -INFINITY;
+  if (none || !(T > 0.f)) {
+    // nothing to draw, or the largest value: its last index
+    int at = -1;
+    if (!none)
+      for (int i = tid; i < len; i += kThreads)
+        if (value(i) == r.zmax) at = lo + i;
+    at = __reduce_max_sync(0xffffffffu, at);
+    __syncthreads();
+    if (tid == 0) sh.last = -1;
+    __syncthreads();
+    if (lane == 0) atomicMax(&sh.last, at);
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int i = 0; i < C; ++i) at = max(at, cluster.map_shared_rank(&sh, i)->last);
+      a.token[row] = at;
+      if (a.logprob) a.logprob[row] = none ? -INFINITY : 0.f;
+    }
+    cluster.sync();  // others' indices are read before they leave
+    return;
+  }
   if (tid == 0)
     sh.task = Task{r,     zrow,  a.token + row, a.logprob ? a.logprob + row : nullptr, u, fmax(1.0 / (double)T, 1e-300),
                    top_p, min_p, n,             top_k};
   if (top_k <= 0 && !(top_p < 1.f) && !(min_p > 0.f)) {
     // ---- no filter: the draw is in index order. Every warp sums a run of
     // its CTA's share; the one that holds the target walks its run again
-    const int run = ((len + kThreads / 32 - 1) / (kThreads / 32) + 31) & ~31, w0 = min(len, warp * run), w1 = min(len, w0 + run);
+    const int run = ((len + kThreads / 32 - 1) / (kThreads / 32) + 127) & ~127, w0 = min(len, warp * run), w1 = min(len, w0 + run);
     u64 m = 0;
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32) m += to_mass(r, weight(r, value(i)));
+    for (int i = w0 + 4 * lane; i < w1; i += 128) {
+      const float4 v = four(i);
+      m += to_mass(r, weight(r, v.x)) + to_mass(r, weight(r, v.y)) + to_mass(r, weight(r, v.z)) + to_mass(r, weight(r, v.w));
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
     if (lane == 0) sh.red[warp] = m;
@@ -694,28 +704,28 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   u64 *boss_list = cluster.map_shared_rank(list, 0);
   auto depth = [&](float z) { return z == r.zmax ? 0.f : r.zmax - z; };
   // the bucket of z, or (level 1) its place among the 2048 parts of bucket
-  // b0; -1: not there. Both rise with falling z.
+  // b0; -1: not there (nor is a NaN). Both rise with falling z.
   auto bucket = [&](float z, int level, int b0) {
+    if (z != z) return -1;
     const float d = depth(z);
     const int b = min(kBuckets - 1, (int)(d * scale));
     if (level == 0) return b;
     return b == b0 ? min(kBuckets - 1, max(0, (int)(fmaf(d, scale, -(float)b0) * kBuckets))) : -1;
   };
-  // f(index of the first, values, whether there is one) for every kBatch
-  // tokens of a thread: loaded together, ahead of what f writes
-  constexpr int kBatch = PER_SM == 1 ? 4 : 2;
-  auto batches = [&](auto f) {
-    for (int i0 = 0; i0 < len; i0 += kBatch * kThreads) {
-      float z[kBatch];
-      bool in[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = i0 + j * kThreads + tid;
-        in[j] = i < len;
-        z[j] = in[j] ? value(i) : -INFINITY;
-      }
-      f(i0 + tid, z, in);
-    }
+  // a value below which no token of the buckets before `end` lies, with room
+  // for the roundings above
+  auto edge = [&](int level, int b0, int end) {
+    const float e = level ? (float)b0 + (float)end / kBuckets : (float)end;
+    if (!level && end >= kBuckets) return -INFINITY;
+    const float d = (e + 0.01f) * 1.001f / scale;
+    const float x = r.zmax - d - fabsf(r.zmax) * 1e-5f;
+    return x == x ? x : -INFINITY;  // (an infinite maximum)
+  };
+  // f(index of the first, values) for every four neighbouring tokens of a
+  // thread, loaded together, ahead of what f writes; behind the last token
+  // the value is NaN, which no bucket and no sum takes
+  auto fours = [&](auto f) {
+    for (int i = 4 * tid; i < len; i += 4 * kThreads) f(i, four(i));
   };
   int cmd = kHist, level = 0, b0 = 0, glo = 0, ghi = 0;
   bool masses = top_p < 1.f || top_k <= 0 || top_k > kList / 2 || min_p > 0.f;  // the first pass sums them all
@@ -733,19 +743,20 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
       u64 m = 0;
       int above = 0;
       const bool sums = masses && level == 0;
-      batches([&](int, const float (&z)[kBatch], const bool (&in)[kBatch]) {
-        int b[kBatch];
-        double w[kBatch];
+      fours([&](int, float4 v) {
+        const float z[4] = {v.x, v.y, v.z, v.w};
+        int b[4];
+        double w[4];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          b[j] = in[j] ? bucket(z[j], level, b0) : -1;
-          if (sums) w[j] = weight(r, z[j]);  // of -inf where there is no token: 0
+        for (int j = 0; j < 4; ++j) {
+          b[j] = bucket(z[j], level, b0);
+          if (sums) w[j] = weight(r, z[j]);
         }
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+        for (int j = 0; j < 4; ++j) {
           if (sums) {
             m += to_mass(r, w[j]);
-            above += w[j] >= (double)min_p;
+            above += w[j] >= (double)min_p;  // (counted only where min_p > 0)
           }
           if (b[j] >= 0) atomicAdd(&hcount[b[j]], 1);
         }
@@ -760,22 +771,18 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
       if (lane < kWindow) sh.parts[warp][lane] = 0;
       __syncwarp();
       u64 m = 0;
-      batches([&](int, const float (&z)[kBatch], const bool (&in)[kBatch]) {
-        int b[kBatch];
-        bool any = false;
+      const float low = edge(level, b0, glo + kWindow);
+      fours([&](int, float4 v) {
+        if (!(v.x >= low || v.y >= low || v.z >= low || v.w >= low)) return;
+        const float z[4] = {v.x, v.y, v.z, v.w};
+        u64 x[4];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          b[j] = in[j] ? bucket(z[j], level, b0) : -1;
-          b[j] = b[j] < 0 ? kWindow : b[j] - glo;
-          any |= b[j] < kWindow;
-        }
-        if (__any_sync(0xffffffffu, any)) {
-          u64 x[kBatch];
+        for (int j = 0; j < 4; ++j) x[j] = to_mass(r, weight(r, z[j]));
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) x[j] = to_mass(r, weight(r, z[j]));
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j)
-            if (b[j] < 0) m += x[j]; else if (b[j] < kWindow && x[j]) atomicAdd(&sh.parts[warp][b[j]], x[j]);
+        for (int j = 0; j < 4; ++j) {
+          int b = bucket(z[j], level, b0);
+          b = b < 0 ? kWindow : b - glo;
+          if (b < 0) m += x[j]; else if (b < kWindow && x[j]) atomicAdd(&sh.parts[warp][b], x[j]);
         }
       });
       m = block_sum(m, sh);
@@ -786,28 +793,27 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
         sh.window[tid] = t;
       }
     } else {  // kGather: count, take places in the leader's list, write
+      const float low = edge(level, b0, ghi + 1);
+      auto in = [&](float z) {
+        if (!(z >= low)) return false;
+        const int b = bucket(z, level, b0);
+        return b >= glo && b <= ghi;
+      };
       int hits = 0;
-      batches([&](int, const float (&z)[kBatch], const bool (&in)[kBatch]) {
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int b = in[j] ? bucket(z[j], level, b0) : -1;
-          hits += b >= glo && b <= ghi;
-        }
-      });
+      fours([&](int, float4 v) { hits += in(v.x) + in(v.y) + in(v.z) + in(v.w); });
       int p = (int)block_before((u64)hits, sh);
       if (tid == kThreads - 1) sh.place = p + hits ? atomicAdd(&boss->listed, p + hits) : 0;
       __syncthreads();
       p += sh.place;
-      if (__any_sync(0xffffffffu, hits))
-        batches([&](int i, const float (&z)[kBatch], const bool (&in)[kBatch]) {
+      if (hits)
+        fours([&](int i, float4 v) {
+          const float z[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            const int b = in[j] ? bucket(z[j], level, b0) : -1;
-            if (b >= glo && b <= ghi) {
-              if (p < kList) boss_list[p] = (u64)ordered(z[j]) << 32 | (0xffffffffu - (uint32_t)(lo + i + j * kThreads));
+          for (int j = 0; j < 4; ++j)
+            if (in(z[j])) {
+              if (p < kList) boss_list[p] = (u64)ordered(z[j]) << 32 | (0xffffffffu - (uint32_t)(lo + i + j));
               ++p;
             }
-          }
         });
     }
     cluster.sync();
