@@ -431,8 +431,9 @@ ifx_status ifx_op_kv4_load(int type, const void *pages, size_t n_pages,
  * sees all kv_len rows, the one before it one less, and so on; with
  * window > 0 each sees its last `window` rows only. softmax(scale q k) v in
  * f32 throughout; a row that sees nothing (kv_len 0, or a query row before
- * the cache's first) gives 0, and rows of out behind the last sequence's are
- * left as they were. A table entry outside the pages hides its rows. At most
+ * the cache's first) gives 0; rows of out that are no sequence's (before
+ * q_start[0], behind q_start[n_seqs]) are left as they were, or set to 0 with
+ * zero_rest. A table entry outside the pages hides its rows. At most
  * IFX_KV4_ATTENTION_MAX_SEQS sequences.
  * ws: scratch of at least ifx_kv4_attention_workspace bytes, 256-byte
  * aligned, any contents, for one call at a time. */
@@ -445,7 +446,8 @@ ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride,
                                 size_t n_seqs, size_t n_heads,
                                 size_t n_kv_heads, size_t head_dim, float scale,
                                 size_t window, void *out, size_t out_stride,
-                                void *ws, size_t ws_bytes, void *stream);
+                                int zero_rest, void *ws, size_t ws_bytes,
+                                void *stream);
 
 /* The next token of every row of logits [rows, n] (rows `stride` values
  * apart, n at most IFX_SAMPLE_ROWS_MAX): Sampler::sample's rule
@@ -461,8 +463,9 @@ ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride,
  * row without any other gives token -1 and logprob -inf. NULL settings:
  * temperature 1, no filter. logprob (nullable): the logarithm of the drawn
  * token's share of the kept mass (0 when greedy). Masses are summed as
- * 64-bit integers (weights to 2^-45 at 128k tokens, 2^-61 at one), so the
- * result does not depend on the order of additions. */
+ * 64-bit integers (weights to 2^-45 for 128256 tokens, to 2^-50 for 2048 and
+ * below), so the result does not depend on the order of additions. Settings
+ * that are NaN are off. */
 #define IFX_SAMPLE_ROWS_MAX (1 << 24)
 ifx_status ifx_op_sample_rows(const float *logits, size_t stride, size_t rows,
                               size_t n, const float *u,

@@ -146,8 +146,8 @@ extern "C" {
                                 max_pages: usize, kv_len: *const i32, q_start: *const i32,
                                 n_seqs: usize, n_heads: usize, n_kv_heads: usize,
                                 head_dim: usize, scale: f32, window: usize, out: *mut c_void,
-                                out_stride: usize, ws: *mut c_void, ws_bytes: usize,
-                                stream: *mut c_void) -> c_int;
+                                out_stride: usize, zero_rest: c_int, ws: *mut c_void,
+                                ws_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn ifx_op_sample_rows(logits: *const f32, stride: usize, rows: usize, n: usize,
                               u: *const f32, temperature: *const f32, top_k: *const i32,
                               top_p: *const f32, min_p: *const f32, token: *mut i32,

@@ -145,7 +145,7 @@ def _load():
         "ifx_op_kv4_load": (st, [C.c_int, vp, sz, sz, sz, vp, sz, vp, vp, vp]),
         "ifx_kv4_attention_workspace": (sz, [sz, sz, sz]),
         "ifx_op_kv4_attention": (st, [C.c_int, vp, sz, sz, vp, sz, vp, sz, vp, vp, sz, sz, sz, sz,
-                                      C.c_float, sz, vp, sz, vp, sz, vp]),
+                                      C.c_float, sz, vp, sz, C.c_int, vp, sz, vp]),
         "ifx_op_sample_rows": (st, [vp, sz, sz, sz, vp, vp, vp, vp, vp, vp, vp, vp]),
         "ifx_kquant_from_ggml": (st, [C.c_uint32, vp, sz, vp, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
         "ifx_tokenizer_load": (st, [C.c_char_p, C.POINTER(vp)]),

@@ -203,6 +203,18 @@ __device__ __forceinline__ void write4(const Kv4AttnArgs &a, long long row, int 
   }
 }
 
+// Zeros into the rows of no sequence, shared out over the grid; by one warp of
+// every CTA, whose reads of q_start overlap the others' work.
+__device__ __forceinline__ void zero_rest(const Kv4AttnArgs &a) {
+  const int lane = threadIdx.x & 31, vals = a.H * a.hd;
+  const auto zeros = [&](int64_t begin, int64_t end) {
+    for (int64_t row = begin + blockIdx.x; row < end; row += gridDim.x)
+      for (int c = 4 * lane; c < vals; c += 128) write4(a, row, c, make_float4(0.f, 0.f, 0.f, 0.f));
+  };
+  zeros(0, min(a.rows, (int64_t)__ldg(a.q_start)));
+  zeros(max(0, __ldg(a.q_start + a.n_seqs)), a.rows);
+}
+
 // Row of q and out of column pair `p` of a segment, or -1.
 template <int PAIRS>
 __device__ __forceinline__ long long pair_row(const Kv4AttnArgs &a, int q0, int ql, int ct, int p, int *head) {
@@ -265,6 +277,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
     fence_mbar_init();
   }
   pdl_launch();
+  if (a.zero_rest && warp == 1) zero_rest(a);
   if (tid < 2 * NW) s_seq[tid][0] = -1;
   // units of every sequence, summed
   if (!a.alone) {
@@ -879,6 +892,7 @@ __global__ void __launch_bounds__(kChunkThreads, ChunkSmem<NB>::kPerSm) kv4_attn
     fence_mbar_init();
   }
   pdl_launch();
+  if (a.zero_rest && warp == 1) zero_rest(a);
   {
     const int n = a.n_seqs, per = (n + kChunkThreads - 1) / kChunkThreads, b0 = min(n, tid * per), b1 = min(n, b0 + per);
     long long mine = 0;

@@ -292,7 +292,7 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
     glo = max(0, min(b, kBuckets - 1) - kWindow / 2);
     next = kMass;
   };
-  int bk = kBuckets;  // the bucket in which the count reaches k.k_eff
+  int bk = kBuckets;  // the bucket in which the count reaches k_eff
   if (cmd == kHist) {
     // the cluster's counts, running sums in place, and the guessed masses
     int c[kPer] = {};
@@ -477,7 +477,7 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
     const u64 before = k.mbase + block_before(ms, sh);
     bool cut = true;
     if (!k.drawing) {
-      // how many are k.kept, and their mass
+      // how many are kept, and their mass
       const u64 room = k.k_eff - min(k.k_eff, k.cbase);
       u64 keep = min(room, (u64)cnt), run = before;
       if (tid == 0) sh.pick = kList + 1;
@@ -539,6 +539,7 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
     sh.lo = glo;
     sh.hi = ghi;
     sh.masses = masses;
+    sh.first = 0;
     sh.listed = 0;
   }
 }
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   };
 
   const float T = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f;
-  const float min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f, u_row = a.u[row];
+  const float want_p = a.min_p ? a.min_p[row] : 0.f, min_p = want_p > 0.f ? fminf(want_p, 1.f) : 0.f, u_row = a.u[row];
   const int top_k = a.top_k ? a.top_k[row] : 0;
   if (tid < 32) sh.pow2[tid] = kPow2[tid];
   if (tid == 0) sh.best = 0;

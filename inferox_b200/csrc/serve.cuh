@@ -101,6 +101,7 @@ struct Kv4AttnArgs {
   int max_pages, n_seqs, H, G, hd, window;
   float scale;
   void *ws;
+  bool zero_rest = false;     // rows of out that are no sequence's become 0
   bool alone = false;         // set by the launch: a CTA per segment
 };
 ifx_status op_kv4_attention(const Kv4AttnArgs &a, cudaStream_t st);

@@ -114,14 +114,14 @@ size_t ifx_kv4_attention_workspace(size_t n_heads, size_t n_kv_heads, size_t hea
 ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride, size_t rows, const void *pages,
                                 size_t n_pages, const int32_t *table, size_t max_pages, const int32_t *kv_len,
                                 const int32_t *q_start, size_t n_seqs, size_t n_heads, size_t n_kv_heads,
-                                size_t head_dim, float scale, size_t window, void *out, size_t out_stride, void *ws,
-                                size_t ws_bytes, void *stream) {
+                                size_t head_dim, float scale, size_t window, void *out, size_t out_stride,
+                                int zero_rest, void *ws, size_t ws_bytes, void *stream) {
   IFX_TRY(check_kv4(type, n_pages, n_kv_heads, head_dim, "kv4_attention"));
   if (!n_heads || n_heads > 65536 || n_heads % n_kv_heads)
     return fail(IFX_ERR_SHAPE, "kv4_attention: query heads must be a multiple of the kv heads");
   if (!q_start && rows != n_seqs) return fail(IFX_ERR_SHAPE, "kv4_attention: one row per sequence without q_start");
-  if (!rows || !n_seqs) return IFX_OK;
-  if (!q || !out || !kv_len || (max_pages && !table) || (n_pages && !pages)) return bad("kv4_attention: null");
+  if (!rows || (!n_seqs && !zero_rest)) return IFX_OK;
+  if (!q || !out || (n_seqs && (!kv_len || (max_pages && !table))) || (n_pages && !pages)) return bad("kv4_attention: null");
   const size_t w = n_heads * head_dim, ts = type_size(type);
   if (q_stride < w || out_stride < w) return fail(IFX_ERR_SHAPE, "kv4_attention: rows overlap");
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(pages, 16) || q_stride * ts % 16 || out_stride * ts % 16)
@@ -131,10 +131,14 @@ ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride, size_t
   if (!(scale == scale) || scale - scale != 0.f) return bad("kv4_attention: scale is not finite");
   if (ws_bytes < kv4_attention_ws((int)n_heads, (int)n_kv_heads, (int)head_dim) || (ws_bytes && (!ws || !aligned(ws, 256))))
     return bad("kv4_attention: workspace too small or not 256-byte aligned");
+  if (!n_seqs) {
+    IFX_CUDA(cudaMemset2DAsync(out, out_stride * ts, 0, w * ts, rows, S(stream)));
+    return IFX_OK;
+  }
   Kv4AttnArgs a{q, out, type, (int64_t)q_stride, (int64_t)out_stride, (int64_t)rows,
                 static_cast<const uint8_t *>(pages), (int64_t)n_pages, table, kv_len, q_start, (int)max_pages,
                 (int)n_seqs, (int)n_heads, (int)n_kv_heads, (int)head_dim,
-                (int)(window > kIntMax ? 0 : window), scale, ws};
+                (int)(window > kIntMax ? 0 : window), scale, ws, zero_rest != 0 && q_start};
   return op_kv4_attention(a, S(stream));
 }
 

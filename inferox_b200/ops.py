@@ -320,9 +320,9 @@ def kv4_attention(q, pages, table, kv_len, n_kv_heads: int, q_start=None, scale=
     them, in the pages table[b]; its query rows are q_start[b]:q_start[b + 1],
     or row b when q_start is None. scale: 1 / sqrt(head_dim) when None;
     window > 0: each row sees its last `window` rows. A row that sees nothing
-    gives 0; rows of `out` behind the last sequence's stay as they were (a
-    fresh `out` is zeroed when q_start is given). workspace: uint8 scratch kept
-    by the caller (kv4_workspace), for one call at a time."""
+    gives 0; rows of a given `out` that are no sequence's stay as they were,
+    those of a fresh one are 0. workspace: uint8 scratch kept by the caller
+    (kv4_workspace), for one call at a time."""
     rows, h, d, qs = _rows("kv4_attention", q)
     n = kv_len.numel()
     if n_kv_heads <= 0 or h % n_kv_heads:
@@ -338,8 +338,9 @@ def kv4_attention(q, pages, table, kv_len, n_kv_heads: int, q_start=None, scale=
         _ints("kv4_attention", q_start)
         _need(q_start.numel() == n + 1, "kv4_attention: q_start is [n_seqs + 1]")
         starts = q_start.data_ptr()
-    if out is None:
-        out, os = (torch.empty if starts is None else torch.zeros)((rows, h, d), dtype=q.dtype, device=q.device), h * d
+    fresh = out is None
+    if fresh:
+        out, os = torch.empty((rows, h, d), dtype=q.dtype, device=q.device), h * d
     else:
         _need(out.shape == q.shape and out.dtype is q.dtype, "kv4_attention: out mismatch")
         os = _rows("kv4_attention", out)[3]
@@ -349,7 +350,8 @@ def kv4_attention(q, pages, table, kv_len, n_kv_heads: int, q_start=None, scale=
         q, pages, table, kv_len, out, workspace, q_start)
     _call(dev, "kv4_attention", lib.ifx_op_kv4_attention, _TYPES[q.dtype], q.data_ptr(), qs, rows, pages.data_ptr(),
           np_, table.data_ptr(), table.shape[1], kv_len.data_ptr(), starts, n, h, n_kv_heads, d,
-          d ** -0.5 if scale is None else scale, window, out.data_ptr(), os, workspace.data_ptr(), workspace.numel())
+          d ** -0.5 if scale is None else scale, window, out.data_ptr(), os, fresh, workspace.data_ptr(),
+          workspace.numel())
     return out
 
 

@@ -249,6 +249,31 @@ def test_attention_empty_rows_and_gaps():
     assert not got[7].any()
 
 
+@pytest.mark.parametrize("ql,seqs", [(1, 3), (2, 3), (70, 20)])  # a row, some rows, chunks of rows
+def test_attention_fresh_out_rows_of_no_sequence(ql, seqs):
+    """Rows before the first sequence's and behind the last's are 0 in an out
+    that the call makes (its memory held sevens), and kept in a given one."""
+    H, G, hd, lead, rest = 8, 8, 64, 4, 300
+    lens = [80 + 3 * i for i in range(seqs)]
+    pages, table, _, _ = filled(np.random.default_rng(3), lens, G, hd)
+    start, rows = i32(lead + ql * np.arange(seqs + 1)), lead + ql * seqs + rest
+    for dtype in (torch.float32, torch.float16):
+        q = torch.randn(rows, H, hd, device=DEV, dtype=dtype)
+        ws = ops.kv4_workspace(H, G, hd)
+        given = torch.full_like(q, 7.0)
+        ops.kv4_attention(q, pages, i32(table), i32(lens), G, q_start=start, out=given, workspace=ws)
+        assert (given[:lead] == 7).all() and (given[-rest:] == 7).all()
+        sevens = torch.full_like(q, 7.0)
+        del sevens
+        got = ops.kv4_attention(q, pages, i32(table), i32(lens), G, q_start=start, workspace=ws)
+        assert not got[:lead].any() and not got[-rest:].any()
+        assert torch.equal(got[lead:-rest], given[lead:-rest])
+        sevens = torch.full_like(q, 7.0)
+        del sevens
+        none = i32(np.zeros((0, 2)))
+        assert not ops.kv4_attention(q, pages, none, i32([]), G, q_start=i32([0]), workspace=ws).any()
+
+
 @pytest.mark.parametrize("amp,scale", [(1e4, 1e-6), (1e-6, 1e3), (30.0, None), (1.0, 0.0), (1.0, -0.3)])
 def test_attention_magnitudes(amp, scale):
     check_attention([70, 150], [1, 1], 8, 2, 128, amp=amp, scale=scale)

@@ -58,7 +58,7 @@ def test_load(kw, want):
 def attn(ty=0, q=P, qs=4096, rows=2, pages=P, np_=4, table=P, mp=4, kl=P, qstart=None, n=2, h=32, g=8, d=128, scale=0.1,
          window=0, out=Q, os=4096, ws=P, wsb=1 << 40):
     return name(lib.ifx_op_kv4_attention(ty, q, qs, rows, pages, np_, table, mp, kl, qstart, n, h, g, d, scale, window,
-                                         out, os, ws, wsb, None))
+                                         out, os, 0, ws, wsb, None))
 
 
 @pytest.mark.parametrize("kw,want", [
