@@ -34,54 +34,13 @@
 // (2.9 TB/s of pages), one of 128k 53 us (2.9 TB/s); one of 1k 13 us, latency.
 #include <algorithm>
 
-#include "serve.cuh"
+#include "kv4_attention.cuh"
 
 namespace ifx {
 
+using namespace kv4;
+
 namespace {
-
-// Scratch in global memory: per CTA two partial results and where its range
-// of tiles begins.
-struct RangeInfo {
-  long long begin, end;  // the segment that holds the CTA's first unit
-  long long total;       // units of the launch
-  int seq, h, ct, live;  // live: CTAs that share them (0: this one has none)
-};
-
-// The units dealt out evenly over `live` CTAs.
-struct Deal {
-  long long each;
-  int more, live;  // the first `more` CTAs have one unit more
-  __device__ __forceinline__ Deal(long long total, int l) : live(l) {
-    each = total >> 32 ? total / l : (uint32_t)total / (uint32_t)l;
-    more = (int)(total - each * l);
-  }
-  __device__ __forceinline__ long long begin(int c) const { return each * c + min(c, more); }
-  __device__ __forceinline__ int owner(long long u) const {  // the CTA that has unit u
-    const long long cut = (each + 1) * more;
-    return u < cut ? (int)(u / (each + 1)) : more + (int)((u - cut) / each);
-  }
-};
-
-template <int N>
-__device__ __forceinline__ void ld_words(const uint8_t *p, uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const uint2 v = reinterpret_cast<const uint2 *>(p)[i];
-      w[2 * i] = v.x, w[2 * i + 1] = v.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-  }
-}
 
 template <int N>
 __device__ __forceinline__ void ld_scales(const uint8_t *p, float (&d)[N]) {
@@ -103,12 +62,6 @@ __device__ __forceinline__ void ld_scales(const uint8_t *p, float (&d)[N]) {
 __device__ __forceinline__ uint32_t movm_trans(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -147,86 +100,6 @@ __device__ __forceinline__ float quad_rows_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-}
-
-// A sequence's share of the work: every (kv head, column tile) is a segment
-// of `units` pages, the first of them page `lo`.
-struct Seq {
-  int len, ql, q0, lo, units, nct;
-};
-template <int PAIRS>
-__device__ __forceinline__ Seq sequence(const Kv4AttnArgs &a, int b) {
-  Seq s;
-  s.len = max(__ldg(a.kv_len + b), 0);
-  if (s.len / kKv4PageRows >= a.max_pages) s.len = min(s.len, a.max_pages * kKv4PageRows);
-  s.q0 = a.q_start ? __ldg(a.q_start + b) : b;
-  s.ql = a.q_start ? (int)min(a.rows, (int64_t)max(0, __ldg(a.q_start + b + 1) - s.q0)) : 1;
-  s.lo = a.window ? (int)(max((int64_t)0, (int64_t)s.len - s.ql - a.window + 1) / kKv4PageRows) : 0;
-  // a sequence without rows still has its zeros to write
-  s.units = max(1, (s.len + kKv4PageRows - 1) / kKv4PageRows - s.lo);
-  s.nct = (int)(((uint32_t)s.ql * (uint32_t)(a.H / a.G) + PAIRS - 1) / PAIRS);
-  return s;
-}
-
-struct Segment {
-  int seq, h, ct, lo, len, ql, q0;
-  long long begin, end;  // in units of the whole launch
-};
-
-template <int PAIRS>
-__device__ __forceinline__ Segment locate(const Kv4AttnArgs &a, const long long *pre, long long u) {
-  int lo = 0, hi = a.n_seqs - 1;  // the last sequence that begins at or before u
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= u) lo = mid; else hi = mid - 1;
-  }
-  const Seq s = sequence<PAIRS>(a, lo);
-  const long long d = u - pre[lo];
-  const long long i = d >> 32 ? d / s.units : (uint32_t)d / (uint32_t)s.units;
-  Segment g;
-  g.seq = lo;
-  g.h = i >> 32 ? (int)(i / s.nct) : (int)((uint32_t)i / (uint32_t)s.nct);
-  g.ct = (int)(i - (long long)g.h * s.nct);
-  g.lo = s.lo;
-  g.len = s.len;
-  g.ql = s.ql;
-  g.q0 = s.q0;
-  g.begin = pre[lo] + i * s.units;
-  g.end = g.begin + s.units;
-  return g;
-}
-
-__device__ __forceinline__ void write4(const Kv4AttnArgs &a, long long row, int col, float4 o) {
-  if (a.type == IFX_TYPE_F16) {
-    const __half2 x = __floats2half2_rn(o.x, o.y), y = __floats2half2_rn(o.z, o.w);
-    *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + row * a.out_stride + col) =
-        make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
-  } else {
-    *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + row * a.out_stride + col) = o;
-  }
-}
-
-// Zeros into the rows of no sequence, shared out over the grid; by one warp of
-// every CTA, whose reads of q_start overlap the others' work.
-__device__ __forceinline__ void zero_rest(const Kv4AttnArgs &a) {
-  const int lane = threadIdx.x & 31, vals = a.H * a.hd;
-  const auto zeros = [&](int64_t begin, int64_t end) {
-    for (int64_t row = begin + blockIdx.x; row < end; row += gridDim.x)
-      for (int c = 4 * lane; c < vals; c += 128) write4(a, row, c, make_float4(0.f, 0.f, 0.f, 0.f));
-  };
-  zeros(0, min(a.rows, (int64_t)__ldg(a.q_start)));
-  zeros(max(0, __ldg(a.q_start + a.n_seqs)), a.rows);
-}
-
-// Row of q and out of column pair `p` of a segment, or -1.
-template <int PAIRS>
-__device__ __forceinline__ long long pair_row(const Kv4AttnArgs &a, int q0, int ql, int ct, int p, int *head) {
-  const int grp = a.H / a.G;
-  const uint32_t e = (uint32_t)ct * PAIRS + p;  // below rows * grp, which the entry point bounds
-  const int tok = (int)(e / (uint32_t)grp);
-  *head = (int)(e - (uint32_t)tok * grp);
-  const long long row = (long long)q0 + tok;
-  return tok < ql && row >= 0 && row < a.rows ? row : -1;
 }
 
 template <int NB, int NT, int NW>
@@ -836,486 +709,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_attn_join_kernel(const __gri
   }
 }
 
-// ------------------------------------------------------------------ chunks
-// Many query rows per kv head (a prompt in chunks, long drafts): a CTA takes
-// 64 of them (query heads times new rows), 16 a warp, against page after
-// page. Each page is unpacked once for the 64 rows, into shared memory as
-// f16: keys as the integers n - 8, which f16 holds exactly, values as
-// (n - 8) dV in two planes (the product's f16 value and its remainder; dV
-// times a power of two that puts the page's largest at 2^14). Queries and
-// probabilities are two f16 planes too, so
-//   scores: per block of 32, (q_hi + q_lo) . (n - 8), then times dK in f32
-//   output: p_hi v_hi + p_lo v_hi + p_hi v_lo
-// with f32 sums: two and three m16n8k16 products where f16 arithmetic would
-// take one each. Bound by the tensor cores' m16n8k16 rate (1.1 ns per SM).
-// The dimensions of a block of eight stand in the order 0 4 1 5 2 6 3 7, as
-// the masks of a key word give them, in keys and queries alike.
-constexpr int kChunkRows = 64, kChunkThreads = 128;
-
-template <int NB>
-struct ChunkSmem {
-  static constexpr int HD = 32 * NB, kStride = HD + 8;  // halves; rows 16 bytes apart modulo 128
-  static constexpr int kRaw = 4 * Kv4Layout::tile_bytes(NB), kPlane = 64 * kStride * 2;
-  static constexpr int kK = 2 * kRaw, kVh = kK + kPlane, kVl = kVh + kPlane, kQh = kVl + kPlane, kQl = kQh + kPlane;
-  static constexpr int kDk = kQl + kPlane, kBar = kDk + 2 * 64 * NB * 4, kBytes = kBar + 16;
-  static constexpr int kPart = kChunkRows * (HD + 2) * 4;
-  static constexpr int kPerSm = NB <= 2 ? 3 : NB <= 4 ? 2 : 1;
-  static_assert(kBytes + (kMaxAttnSeqs + 1) * 8 <= 227 * 1024, "shared memory of one CTA");
-};
-
-__device__ __forceinline__ uint32_t h2(__half2 x) { return *reinterpret_cast<const uint32_t *>(&x); }
-__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); }
-
-// The pair (n, n') of f16 subnormals n * 2^-24 as n - 8, n' - 8: one fused
-// multiply-add in f16, exact (in steps of 2^-9, to keep the factor in range;
-// nibbles at bits 4..7 come 16 times larger).
-__device__ __forceinline__ __half2 nibble_pair(uint32_t w, bool high) {
-  const uint32_t m = high ? w & 0x00f000f0u : w & 0x000f000fu;
-  return __hfma2(as_h2(m), __float2half2_rn(high ? 2048.f : 32768.f), __float2half2_rn(-8.f / 512.f));
-}
-
-template <int NB>
-__global__ void __launch_bounds__(kChunkThreads, ChunkSmem<NB>::kPerSm) kv4_attn_chunk_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  using L = ChunkSmem<NB>;
-  constexpr int HD = L::HD, LD = L::kStride, TB = Kv4Layout::tile_bytes(NB), ROWS = kChunkRows;
-  extern __shared__ __align__(128) uint8_t sm[];
-  __half *Ks = reinterpret_cast<__half *>(sm + L::kK), *Vh = reinterpret_cast<__half *>(sm + L::kVh),
-         *Vl = reinterpret_cast<__half *>(sm + L::kVl), *Qh = reinterpret_cast<__half *>(sm + L::kQh),
-         *Ql = reinterpret_cast<__half *>(sm + L::kQl);
-  float *dk2 = reinterpret_cast<float *>(sm + L::kDk);  // [2][64][NB], page by page
-  uint64_t *bar = reinterpret_cast<uint64_t *>(sm + L::kBar);
-  long long *pre = reinterpret_cast<long long *>(sm + L::kBytes);
-  __shared__ long long s_scan[kChunkThreads / 32];
-  __shared__ float s_q[ROWS];  // a query row's factor for its scores
-  __shared__ uint32_t s_top[2][kChunkThreads / 32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  if (tid == 0) {
-    mbar_init(&bar[0], 1);
-    mbar_init(&bar[1], 1);
-    fence_mbar_init();
-  }
-  pdl_launch();
-  if (a.zero_rest && warp == 1) zero_rest(a);
-  {
-    const int n = a.n_seqs, per = (n + kChunkThreads - 1) / kChunkThreads, b0 = min(n, tid * per), b1 = min(n, b0 + per);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) {
-      const Seq s = sequence<ROWS>(a, b);
-      pre[b] = mine;
-      mine += (long long)s.units * s.nct * a.G;
-    }
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += x;
-    }
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    long long base = inc - mine;
-    for (int i = 0; i < warp; ++i) base += s_scan[i];
-    for (int b = b0; b < b1; ++b) pre[b] += base;
-    if (tid == kChunkThreads - 1) pre[n] = base + mine;
-    __syncthreads();
-  }
-  const long long total = pre[a.n_seqs];
-  const int live = (int)min((long long)gridDim.x, (total + 3) / 4);  // four pages or more, for few partials
-  RangeInfo *info = static_cast<RangeInfo *>(a.ws);
-  if ((int)blockIdx.x >= live) {
-    if (tid == 0) info[blockIdx.x].live = 0;
-    return;
-  }
-  const Deal deal(total, live);
-  const long long u0 = deal.begin(blockIdx.x), u1 = deal.begin(blockIdx.x + 1);
-  const int grp = a.H / a.G;
-  Segment s = locate<ROWS>(a, pre, u0);
-  if (tid == 0) info[blockIdx.x] = RangeInfo{s.begin, s.end, total, s.seq, s.h, s.ct, live};
-
-  // thread 0: the copies, one page ahead of the page that is unpacked
-  Segment fs = s;
-  long long fu = u0;
-  auto fetch = [&](int st) {
-    if (fu >= u1) return;
-    if (fu == fs.end) fs = locate<ROWS>(a, pre, fu);
-    const int j = fs.lo + (int)(fu - fs.begin);
-    const int page = j < a.max_pages ? __ldg(a.table + (size_t)fs.seq * a.max_pages + j) : -1;
-    const int tiles = min(4, (fs.len - j * kKv4PageRows + kKv4TileRows - 1) / kKv4TileRows);
-    if ((unsigned)page < (unsigned)a.n_pages && tiles > 0) {
-      mbar_arrive_expect_tx(&bar[st], (uint32_t)(tiles * TB));
-      bulk_g2s(sm + st * L::kRaw, a.pages + ((int64_t)page * a.G + fs.h) * (4 * TB), (uint32_t)(tiles * TB), &bar[st]);
-    } else {
-      mbar_arrive(&bar[st]);
-    }
-    ++fu;
-  };
-  if (tid == 0) {
-    fetch(0);
-    fetch(1);
-  }
-  int st = 0;
-  uint32_t phase = 0;
-  long long u = u0;
-  while (u < u1) {
-    // ---- 64 query rows: two f16 planes each, scaled by a power of two that
-    // puts the row's largest magnitude into [2^10, 2^11)
-    __syncthreads();  // the last segment's products are done
-    for (int r = warp; r < ROWS; r += kChunkThreads / 32) {
-      int head;
-      const long long row = pair_row<ROWS>(a, s.q0, s.ql, s.ct, r, &head);
-      float x[NB];
-      float big = 0.f;
-      bool bad = false;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        x[b] = 0.f;
-        if (row >= 0) {
-          const int64_t at = row * a.q_stride + (s.h * grp + head) * HD + 32 * b + lane;
-          x[b] = a.type == IFX_TYPE_F16 ? __half2float(static_cast<const __half *>(a.q)[at]) : static_cast<const float *>(a.q)[at];
-        }
-        big = fmaxf(big, fabsf(x[b]));
-        bad |= !(fabsf(x[b]) < INFINITY);
-      }
-      big = warp_max(big);
-      const int e = big > 0.f ? min(100, max(-100, 10 + 127 - (int)(__float_as_uint(big) >> 23))) : 0;
-      // the scale's sign goes into the query, so that the factor of the
-      // scores is positive and the largest product is the largest score; a
-      // scale of 0 makes the query 0
-      const float up = a.scale == 0.f ? 0.f : copysignf(__uint_as_float((uint32_t)(127 + e) << 23), a.scale);
-      // dimension i of eight stands at place 2 (i % 4) + i / 4
-      const int place = (lane & ~7) + 2 * (lane & 3) + (lane >> 2 & 1);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const float v = x[b] * up;
-        const __half hi = __float2half_rn(v);
-        Qh[r * LD + 32 * b + place] = hi;
-        Ql[r * LD + 32 * b + place] = __float2half_rn(v - __half2float(hi));
-      }
-      // nibble pairs come in steps of 2^-9
-      const float f = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f * 512.f * __uint_as_float((uint32_t)(127 - e) << 23);
-      bad = __any_sync(0xffffffffu, bad);  // a query that is not finite has scores NaN
-      if (lane == 0) s_q[r] = bad ? __uint_as_float(0x7fc00000u) : f;
-    }
-    __syncthreads();
-    const int r0 = 16 * warp + g;  // this lane's rows r0 and r0 + 8
-    int jmax[2], jmin[2];
-    float qs[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int head;
-      const long long row = pair_row<ROWS>(a, s.q0, s.ql, s.ct, r0 + 8 * i, &head);
-      const int pos = s.len - s.ql + (int)(row - s.q0);
-      jmax[i] = row >= 0 ? pos : INT32_MAX;
-      jmin[i] = row >= 0 && a.window ? max(0, pos - a.window + 1) : 0;
-      qs[i] = s_q[r0 + 8 * i];
-    }
-    const int see_lo = __reduce_max_sync(0xffffffffu, max(jmin[0], jmin[1]));
-    const int see_hi = __reduce_min_sync(0xffffffffu, min(jmax[0], jmax[1]));
-    // the last row that any row of this warp sees, and the first
-    const int top0 = jmax[0] == INT32_MAX ? -1 : jmax[0], top1 = jmax[1] == INT32_MAX ? -1 : jmax[1];
-    const int any_hi = __reduce_max_sync(0xffffffffu, max(top0, top1));
-    const int any_lo = __reduce_min_sync(0xffffffffu, min(jmin[0], jmin[1]));
-    float o[4 * NB][4];
-#pragma unroll
-    for (int i = 0; i < 4 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    int kref = 1000;  // o counts in 2^-(1 + kref) (p times 2^10, nibbles in 2^-9): the smallest page exponent so far
-
-    const long long stop = min(u1, s.end);
-    auto page_at = [&](int j) { return j < a.max_pages ? __ldg(a.table + (size_t)s.seq * a.max_pages + j) : -1; };
-    int coming = page_at(s.lo + (int)(u - s.begin));
-    for (; u < stop; ++u) {
-      const int j = s.lo + (int)(u - s.begin), row0 = j * kKv4PageRows;
-      // the page may be missing: its rows are hidden
-      const int page = coming;
-      if (u + 1 < stop) coming = page_at(j + 1);
-      const bool ok = (unsigned)page < (unsigned)a.n_pages;
-      const int rows_here = ok ? min(kKv4PageRows, max(0, s.len - row0)) : 0;
-      uint8_t *raw = sm + st * L::kRaw;
-      float *dks = dk2 + st * 64 * NB;
-      mbar_wait(&bar[st], phase, nullptr, 0);
-      // ---- unpack: the largest value scale, then keys and values
-      uint32_t top = 0;
-      for (int e = tid; e < 64 * NB; e += kChunkThreads) {
-        const int r = e / NB, b = e % NB;
-        const uint8_t *tb = raw + r / 16 * TB;
-        uint16_t kd = 0, vd = 0;
-        if (r < rows_here) {
-          kd = reinterpret_cast<const uint16_t *>(tb + Kv4Layout::k_scales(NB))[r % 16 * NB + b];
-          vd = reinterpret_cast<const uint16_t *>(tb + Kv4Layout::v_scales(NB))[r % 16 * NB + b];
-        }
-        dks[e] = h2f(kd);
-        top = max(top, (uint32_t)(vd & 0x7fffu));
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) s_top[st][warp] = top;
-      __syncthreads();  // scales are in place, and the last page's products done
-      top = max(max(s_top[st][0], s_top[st][1]), max(s_top[st][2], s_top[st][3]));
-      const float dmax = h2f((uint16_t)min(top, 0x7bffu));
-      const int kpage = top ? 14 + 127 - (int)(__float_as_uint(dmax) >> 23) : 1000;  // dmax 2^kpage in [2^14, 2^15)
-      const float vup = top ? __uint_as_float((uint32_t)(127 + kpage) << 23) : 0.f;
-      for (int e = tid; e < 64 * NB * 4; e += kChunkThreads) {
-        // key words: row r, lane coordinate tt, block b
-        const int b = e % NB, tt = e / NB % 4, r = e / (4 * NB);
-        const uint32_t w = reinterpret_cast<const uint32_t *>(raw + r / 16 * TB)[(r % 16 * 4 + tt) * NB + b], y = w >> 8;
-        const uint4 v = make_uint4(h2(nibble_pair(w, false)), h2(nibble_pair(w, true)), h2(nibble_pair(y, false)), h2(nibble_pair(y, true)));
-        *reinterpret_cast<uint4 *>(Ks + r * LD + 32 * b + 8 * tt) = v;
-      }
-      for (int e = tid; e < 32 * NB * 8; e += kChunkThreads) {
-        // value words: row pair pr, lane coordinate gg, block b
-        const int b = e % NB, gg = e / NB % 8, pr = e / (8 * NB), r = 2 * pr;
-        const uint8_t *tb = raw + r / 16 * TB;
-        const uint32_t w = reinterpret_cast<const uint32_t *>(tb + Kv4Layout::v_words(NB))[(pr % 8 * 8 + gg) * NB + b], y = w >> 8;
-        const __half *sc = reinterpret_cast<const __half *>(tb + Kv4Layout::v_scales(NB)) + r % 16 * NB + b;
-        // dV 2^kpage: exact down to 2^-28 of the page's largest
-        const __half2 d = __floats2half2_rn(r < rows_here ? __half2float(sc[0]) * vup : 0.f,
-                                            r + 1 < rows_here ? __half2float(sc[NB]) * vup : 0.f);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __half2 x = nibble_pair(i < 2 ? w : y, i & 1);
-          const __half2 p = __hmul2(x, d);
-          hi[i] = h2(p);
-          lo[i] = h2(__hfma2(x, d, __hneg2(p)));
-        }
-        const int at = r * LD + 32 * b + 4 * gg;
-        *reinterpret_cast<uint2 *>(Vh + at) = make_uint2(prmt(hi[0], hi[1], 0x5410u), prmt(hi[2], hi[3], 0x5410u));
-        *reinterpret_cast<uint2 *>(Vh + at + LD) = make_uint2(prmt(hi[0], hi[1], 0x7632u), prmt(hi[2], hi[3], 0x7632u));
-        *reinterpret_cast<uint2 *>(Vl + at) = make_uint2(prmt(lo[0], lo[1], 0x5410u), prmt(lo[2], lo[3], 0x5410u));
-        *reinterpret_cast<uint2 *>(Vl + at + LD) = make_uint2(prmt(lo[0], lo[1], 0x7632u), prmt(lo[2], lo[3], 0x7632u));
-      }
-      __syncthreads();
-      if (tid == 0) fetch(st);
-      if (++st == 2) {
-        st = 0;
-        phase ^= 1;
-      }
-      if (row0 > any_hi || row0 + kKv4PageRows <= any_lo || !rows_here) continue;  // nothing for this warp's rows
-      // ---- scores
-      float sc[8][4];
-#pragma unroll
-      for (int n = 0; n < 8; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        uint32_t ah[2][4], al[2][4];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int at = (16 * warp + (lane & 15)) * LD + 32 * b + 16 * k + (lane >> 4) * 8;
-          ldsm_x4(ah[k], smem_u32(Qh + at));
-          ldsm_x4(al[k], smem_u32(Ql + at));
-        }
-#pragma unroll
-        for (int n0 = 0; n0 < 8; n0 += 4) {
-          // keys 8 n .. 8 n + 7, 32 dimensions: two k-steps; four independent sums at a time
-          uint32_t kb[4][4];
-          float acc[4][4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            ldsm_x4(kb[n], smem_u32(Ks + (8 * (n0 + n) + (lane & 7)) * LD + 32 * b + (lane >> 3) * 8));
-            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const uint32_t(&x)[4] = k < 2 ? al[k] : ah[k - 2];
-              mma_16816(acc[n], x[0], x[1], x[2], x[3], kb[n][2 * (k & 1)], kb[n][2 * (k & 1) + 1], acc[n]);
-            }
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float d0 = dks[(8 * (n0 + n) + 2 * t) * NB + b], d1 = dks[(8 * (n0 + n) + 2 * t + 1) * NB + b];
-            sc[n0 + n][0] = fmaf(d0, acc[n][0], sc[n0 + n][0]);
-            sc[n0 + n][1] = fmaf(d1, acc[n][1], sc[n0 + n][1]);
-            sc[n0 + n][2] = fmaf(d0, acc[n][2], sc[n0 + n][2]);
-            sc[n0 + n][3] = fmaf(d1, acc[n][3], sc[n0 + n][3]);
-          }
-        }
-      }
-      float mx[2] = {-INFINITY, -INFINITY};
-      const bool whole = row0 >= see_lo && row0 + kKv4PageRows - 1 <= see_hi;
-      if (!whole) {
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int jj = row0 + 8 * n + 2 * t + (i & 1);
-            if (jj < jmin[i >> 1] || jj > jmax[i >> 1]) sc[n][i] = -INFINITY;
-          }
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        mx[0] = fmaxf(mx[0], fmaxf(sc[n][0], sc[n][1]));
-        mx[1] = fmaxf(mx[1], fmaxf(sc[n][2], sc[n][3]));
-      }
-      // ---- running maximum; the page's exponent
-      float alpha[2], base[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        const float m2 = fmaxf(m[i], mx[i] == -INFINITY ? -INFINITY : mx[i] * qs[i]);
-        base[i] = m2 == -INFINITY ? 0.f : m2;
-        alpha[i] = ex2(m[i] - base[i]);
-        m[i] = m2;
-        l[i] *= alpha[i];
-      }
-      int pf = 10;  // p enters times 2^10, less for a page of smaller values
-      if (kpage < kref) {
-        const float down = kref == 1000 ? 0.f : __uint_as_float((uint32_t)max(0, 127 + kpage - kref) << 23);
-        alpha[0] *= down;
-        alpha[1] *= down;
-        kref = kpage;
-      } else if (kpage > kref) {
-        pf = max(-116, 10 + kref - kpage);
-      }
-      // p 2^pf = exp2(x qs - (base - pf)); its sum is divided by 2^pf again
-      base[0] -= (float)pf;
-      base[1] -= (float)pf;
-      float sum[2] = {0.f, 0.f};
-      // ---- probabilities
-      uint32_t ph[4][4], pl[4][4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float x0 = ex2(fmaf(sc[2 * ks + k][2 * i], qs[i], -base[i]));
-            const float x1 = ex2(fmaf(sc[2 * ks + k][2 * i + 1], qs[i], -base[i]));
-            sum[i] += x0 + x1;
-            const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
-            ph[ks][2 * k + i] = h2(__floats2half2_rn(h0, h1));  // the first 11 bits, exactly
-            pl[ks][2 * k + i] = h2(__floats2half2_rn(x0 - h0, x1 - h1));
-          }
-      // ---- output: a page's sum starts from zero and is added in f32, whose
-      // rounding has no direction (the tensor cores cut their sums off: 40
-      // pages in one accumulator came out 4.8e-6 off, so 4e-7)
-#pragma unroll
-      for (int n = 0; n < 4 * NB; n += 4) {
-        float acc[4][4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          uint32_t vh[2][4], vl[2][4];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int at = (16 * ks + (lane & 15)) * LD + 8 * (n + 2 * q) + (lane >> 4) * 8;
-            ldsm_x4_t(vh[q], smem_u32(Vh + at));
-            ldsm_x4_t(vl[q], smem_u32(Vl + at));
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816(acc[k], pl[ks][0], pl[ks][1], pl[ks][2], pl[ks][3], vh[k >> 1][2 * (k & 1)], vh[k >> 1][2 * (k & 1) + 1], acc[k]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816(acc[k], ph[ks][0], ph[ks][1], ph[ks][2], ph[ks][3], vl[k >> 1][2 * (k & 1)], vl[k >> 1][2 * (k & 1) + 1], acc[k]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816(acc[k], ph[ks][0], ph[ks][1], ph[ks][2], ph[ks][3], vh[k >> 1][2 * (k & 1)], vh[k >> 1][2 * (k & 1) + 1], acc[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[n + k][i] = fmaf(o[n + k][i], alpha[i >> 1], acc[k][i]);
-      }
-      const float back = __uint_as_float((uint32_t)(127 - pf) << 23);
-      l[0] = fmaf(sum[0], back, l[0]);
-      l[1] = fmaf(sum[1], back, l[1]);
-    }
-    // ---- the segment's end, or the range's: the result, or a partial
-    const bool whole = s.begin >= u0 && s.end <= u1;
-    float *part = reinterpret_cast<float *>(static_cast<uint8_t *>(a.ws) + gridDim.x * sizeof(RangeInfo)) +
-                  (size_t)(2 * blockIdx.x + (s.begin <= u0 ? 0 : 1)) * (L::kPart / 4);
-    const float unit = kref == 1000 ? 0.f : __uint_as_float((uint32_t)max(0, 127 - 1 - kref) << 23);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum = l[i];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const int r = r0 + 8 * i;
-      int head;
-      const long long row = pair_row<ROWS>(a, s.q0, s.ql, s.ct, r, &head);
-      const float f = !whole ? unit : sum == 0.f ? 0.f : unit / sum;
-#pragma unroll
-      for (int n = 0; n < 4 * NB; ++n) {
-        const float x = o[n][2 * i] * f, y = o[n][2 * i + 1] * f;
-        const int col = 8 * n + 2 * t;
-        if (!whole) {
-          *reinterpret_cast<float2 *>(part + r * HD + col) = make_float2(x, y);
-        } else if (row >= 0) {
-          const int64_t at = row * a.out_stride + (s.h * grp + head) * HD + col;
-          if (a.type == IFX_TYPE_F16) *reinterpret_cast<__half2 *>(static_cast<__half *>(a.out) + at) = __floats2half2_rn(x, y);
-          else *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at) = make_float2(x, y);
-        }
-      }
-      if (!whole && t == 0) {
-        part[ROWS * HD + r] = m[i];
-        part[ROWS * (HD + 1) + r] = sum;
-      }
-    }
-    if (u < u1) s = locate<ROWS>(a, pre, u);
-  }
-}
-
-// Joins the chunk kernel's partials: block c as in kv4_attn_join_kernel, a
-// warp per query row.
-__global__ void __launch_bounds__(256) kv4_attn_chunk_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  pdl_wait();
-  constexpr int ROWS = kChunkRows;
-  const RangeInfo *info = static_cast<const RangeInfo *>(a.ws);
-  const int c = blockIdx.x + 1, HD = a.hd, grp = a.H / a.G, lane = threadIdx.x & 31;
-  const RangeInfo r = info[c];
-  if (!r.live) return;
-  const Deal deal(r.total, r.live);
-  const long long mine = deal.begin(c), prev = deal.begin(c - 1);
-  if (r.begin >= mine || r.begin < prev) return;
-  const int part = ROWS * (HD + 2);
-  const float *parts = reinterpret_cast<const float *>(static_cast<const uint8_t *>(a.ws) + (gridDim.x + 1) * sizeof(RangeInfo));
-  auto at = [&](int k) { return parts + (size_t)(2 * (c - 1 + k) + (k == 0 && r.begin > prev ? 1 : 0)) * part; };
-  const int n = deal.owner(r.end - 1) - c + 2;
-  const Seq sq = sequence<ROWS>(a, r.seq);
-  // a warp per row
-  for (int p = blockIdx.y * 8 + (threadIdx.x >> 5); p < ROWS; p += 8 * gridDim.y) {
-    int head;
-    const long long row = pair_row<ROWS>(a, sq.q0, sq.ql, r.ct, p, &head);
-    if (row < 0) continue;
-    float M = -INFINITY, S = 0.f;
-    for (int k = lane; k < n; k += 32) M = fmaxf(M, at(k)[ROWS * HD + p]);
-    M = warp_max(M);
-    const float base = M == -INFINITY ? 0.f : M;
-    float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) {
-      const float *pt = at(k);
-      const float w = ex2(pt[ROWS * HD + p] - base);
-      S = fmaf(w, pt[ROWS * (HD + 1) + p], S);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int col = 4 * lane + 128 * i;
-        if (col < HD) {
-          const float4 x = *reinterpret_cast<const float4 *>(pt + p * HD + col);
-          v[i].x = fmaf(w, x.x, v[i].x), v[i].y = fmaf(w, x.y, v[i].y), v[i].z = fmaf(w, x.z, v[i].z), v[i].w = fmaf(w, x.w, v[i].w);
-        }
-      }
-    }
-    const float f = S == 0.f ? 0.f : 1.f / S;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = 4 * lane + 128 * i;
-      if (col < HD) write4(a, row, (r.h * grp + head) * HD + col, make_float4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f));
-    }
-  }
-}
-
-template <int NB>
-ifx_status run_chunk(const Kv4AttnArgs &a, cudaStream_t st) {
-  using L = ChunkSmem<NB>;
-  auto kernel = kv4_attn_chunk_kernel<NB>;
-  static std::atomic<uint64_t> done{0};
-  IFX_TRY(raise_smem(kernel, L::kBytes + (kMaxAttnSeqs + 1) * 8, done));
-  const int grid = kNumSMs * L::kPerSm;
-  kernel<<<grid, kChunkThreads, L::kBytes + ((size_t)a.n_seqs + 1) * sizeof(long long), st>>>(a);
-  IFX_CUDA(cudaGetLastError());
-  IFX_CUDA(launch(kv4_attn_chunk_join_kernel, dim3(grid - 1, kChunkRows / 8), dim3(256), 0, st, true, a));
-  return IFX_OK;
-}
-
 template <int NB, int NT, int NW, int MINB>
 ifx_status run(const Kv4AttnArgs &args, bool alone, cudaStream_t st) {
   using L = Smem<NB, NT, NW>;
@@ -1334,13 +727,7 @@ ifx_status run(const Kv4AttnArgs &args, bool alone, cudaStream_t st) {
 
 template <int NB>
 ifx_status run_nb(const Kv4AttnArgs &a, cudaStream_t st) {
-  // columns per kv head of a sequence, on average (lengths are on the device)
-  const int64_t columns = (a.rows * (a.H / a.G) + a.n_seqs - 1) / a.n_seqs;
-  // 64 columns a CTA pay where they fill the GPU without cutting the axis of
-  // keys into many parts. 128 rows of 4 sequences, 32 heads of 64 on 8, 2600
-  // keys (512 columns, 256 tiles of 64): 120 us against 172 us by eights; 96
-  // columns, 128 tiles: 134 against 141; 192 columns, 24 tiles: 40 against 29
-  if (columns >= 64 && (int64_t)a.n_seqs * a.G * ((columns + 63) / 64) >= 128) return run_chunk<NB>(a, st);
+  const int64_t columns = kv4_columns(a);
   // One row per sequence and short tables: a CTA per segment, whose warps
   // share its pages, and no second kernel. 16 sequences of 460 to 2300 keys,
   // 128 segments: 18 us against 23; 1100 keys: 13.4 us against 13.7, with
@@ -1361,14 +748,11 @@ ifx_status run_nb(const Kv4AttnArgs &a, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv4_attention_ws(int, int, int hd) {
-  // per CTA two partials of 64 query rows (the chunk kernel's; the other's are smaller)
-  const int per_sm = hd <= 64 ? 3 : hd <= 128 ? 2 : 1;
-  return (size_t)per_sm * kNumSMs * (sizeof(RangeInfo) + 2 * kChunkRows * (size_t)(hd + 2) * sizeof(float));
-}
+size_t kv4_attention_ws(int, int, int hd) { return kv4_chunks_ws(hd); }  // (the kernel above needs less)
 
 ifx_status op_kv4_attention(const Kv4AttnArgs &a, cudaStream_t st) {
   if (!a.rows) return IFX_OK;
+  if (kv4_chunks_take(a)) return kv4_attention_chunks(a, st);
   switch (a.hd / 32) {
     case 1: return run_nb<1>(a, st);
     case 2: return run_nb<2>(a, st);

@@ -170,6 +170,53 @@ def test_attention_chunks_of_many_sequences(H, G, hd, window):
     check_attention(lens, qlens, H, G, hd, torch.float16 if hd == 32 else torch.float32, window=window)
 
 
+@pytest.mark.parametrize("hd", range(32, 257, 32))
+@pytest.mark.parametrize("dtype,window", [(torch.float32, 0), (torch.float32, 70), (torch.float16, 0)])
+def test_attention_chunks_every_head_size(hd, dtype, window):
+    """Tiles of 128 query rows: groups of three, lengths from none to many
+    pages, more query rows than cached ones."""
+    H, G = (30, 10) if hd <= 64 else (12, 4)
+    check_attention([290, 40, 0, 130, 30, 777], [90, 1, 0, 130, 64, 17], H, G, hd, dtype, window=window)
+
+
+def test_attention_chunks_whole_prompts_and_one_tile():
+    check_attention([200, 129, 1, 64], [200, 129, 1, 64], 16, 8, 128)  # nothing cached before: each row sees up to itself
+    check_attention([128], [128], 32, 8, 64)
+    check_attention([64] * 12, [64] * 12, 8, 8, 64)  # a page a tile: no partial results
+
+
+def test_attention_chunks_streams_and_graph():
+    """Calls that overlap on two streams, each with its own workspace, and a
+    captured one give the bits of a call alone."""
+    calls = []
+    for seed, (H, G, hd) in enumerate([(32, 8, 64), (16, 4, 128)]):
+        lens = [500, 333, 128, 64]
+        pages, table, _, _ = filled(np.random.default_rng(seed), lens, G, hd)
+        q = torch.randn(4 * 64, H, hd, device=DEV)
+        args = (q, pages, i32(table), i32(lens), G)
+        kw = dict(q_start=i32(64 * np.arange(5)), workspace=ops.kv4_workspace(H, G, hd))
+        calls.append((args, kw, ops.kv4_attention(*args, **kw)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    outs = []
+    for _ in range(8):
+        for st, (args, kw, _) in zip(streams, calls):
+            with torch.cuda.stream(st):
+                outs.append(ops.kv4_attention(*args, **kw))
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, calls[i % 2][2])
+    args, kw, want = calls[0]
+    out = torch.zeros_like(want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.kv4_attention(*args, **kw, out=out)
+    out.fill_(3.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 def test_attention_chunks_gaps_and_magnitudes():
     """The same kernel: a missing page, rows behind the last sequence, a query
     that is not finite, queries and values of very different sizes, a scale
