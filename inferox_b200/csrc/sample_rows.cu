@@ -16,11 +16,11 @@
 //
 // What bounds it. A row is read once (4 n bytes) into the shared memory of a
 // cluster of CTAs, which keeps it for the passes that follow; the weights
-// cost about 20 instructions each, 13 of them in 64-bit floating point (an
+// cost about 20 instructions each, 11 of them in 64-bit floating point (an
 // SM does two warps' worth a clock), which overlap the reads of other rows.
 // One row alone is bound by latency: a cluster barrier takes 1 us. Measured:
-// one row of 32000 16 us; 64 rows of 128256 with all filters 103 us (0.32
-// TB/s of logits); 256 rows without a filter 108 us (1.22 TB/s).
+// one row of 32000 16 us; 64 rows of 128256 with all filters 99 us (0.33
+// TB/s of logits); 256 rows without a filter 103 us (1.28 TB/s).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -61,29 +61,31 @@ __device__ const double kPow2[32] = {  // 2^(j / 32)
     1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
     1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__device__ const double kPow2Fine[4] = {1.0, 1.0054299011128027, 1.0108892860517005, 1.016378314910953};  // 2^(j / 128)
 
 struct Row {
   float zmax;
   double cut;        // this far below the maximum a weight rounds to 0
-  double c, unit;    // 32 log2(e) / T; 2^s
+  float zcut;        // a value from which on below nothing counts
+  double c, unit;    // 128 log2(e) / T; 2^s
   int s;
-  const double *pow2;  // 2^(j / 32), in shared memory
+  const double *pow2;  // 2^(j / 128), in shared memory
 };
 
-// exp((z - zmax) / T) by table and polynomial: with x = (z - zmax) 32 log2(e)
-// / T = 32 n + j + f, |f| <= 1/2, it is 2^n 2^(j/32) e^y, y = f ln2 / 32. Five
-// terms of the series leave y^6 / 720 < 2^-48.
+// exp((z - zmax) / T) by table and polynomial: with x = (z - zmax) 128 log2(e)
+// / T = 128 n + j + f, |f| <= 1/2, it is 2^n 2^(j/128) e^y, y = f ln2 / 128.
+// Four terms of the series leave y^5 / 120 < 2^-49.
 __device__ __forceinline__ double weight(const Row &r, float z) {
   const double d = (double)z - (double)r.zmax;
   const double x = d * r.c;
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
   const double k = x + kRound, f = x - (k - kRound);
-  constexpr double y1 = 0.021660849392498290, y2 = y1 * y1 / 2, y3 = y2 * y1 / 3, y4 = y3 * y1 / 4, y5 = y4 * y1 / 5;
-  const double e = fma(f, fma(f, fma(f, fma(f, fma(f, y5, y4), y3), y2), y1), 1.0);
+  constexpr double y1 = 0.0054152123481245725, y2 = y1 * y1 / 2, y3 = y2 * y1 / 3, y4 = y3 * y1 / 4;
+  const double e = fma(f, fma(f, fma(f, fma(f, y4, y3), y2), y1), 1.0);
   const int i = __double2loint(k);
-  const double t = r.pow2[i & 31] * e;
-  const double w = __hiloint2double(__double2hiint(t) + (i >> 5) * (1 << 20), __double2loint(t));
-  return z == r.zmax ? 1.0 : -d < r.cut ? w : 0.0;
+  const double t = r.pow2[i & 127] * e;
+  const double w = __hiloint2double(__double2hiint(t) + (i >> 7) * (1 << 20), __double2loint(t));
+  return z == r.zmax ? 1.0 : z >= r.zcut ? w : 0.0;
 }
 __device__ __forceinline__ u64 to_mass(const Row &r, double w) {
   // w 2^s <= 2^50: adding 2^52 leaves the rounded integer in the low bits
@@ -115,7 +117,7 @@ struct Task {
 struct Shared {
   Task task;
   Book book;
-  double pow2[32];
+  double pow2[128];
   u64 red[kThreads / 32];
   u64 best;            // this CTA's largest value (ordered bits)
   u64 mass;            // this CTA's mass: of all its tokens, or before the window
@@ -605,25 +607,24 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
       }
     }
   }
-  if (tid < 32) sh.pow2[tid] = kPow2[tid];
+  if (tid < 128) sh.pow2[tid] = kPow2[tid / 4] * kPow2Fine[tid % 4];
   __syncthreads();
   float top = -INFINITY;
   if (IN_SMEM && wide) {
+    // kept as it is: a NaN is in no bucket and has no weight, -0 equals +0
+    // until the sort
     mbar_wait(&bar, 0, nullptr, 0);
-    float4 *own = reinterpret_cast<float4 *>(zs);
 #pragma unroll 4
     for (int i = tid; i < len / 4; i += kThreads) {
-      const float4 w = own[i], v = make_float4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
-      if (__float_as_uint(w.x) != __float_as_uint(v.x) || __float_as_uint(w.y) != __float_as_uint(v.y) ||
-          __float_as_uint(w.z) != __float_as_uint(v.z) || __float_as_uint(w.w) != __float_as_uint(v.w))
-        own[i] = v;
+      const float4 v = reinterpret_cast<const float4 *>(zs)[i];
       top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
     for (int i = (len & ~3) + tid; i < len; i += kThreads) {
-      const float z = clean(zrow[lo + i]);
+      const float z = zrow[lo + i];
       zs[i] = z;
       top = fmaxf(top, z);
     }
+    top += 0.f;
   } else if (wide) {
     const float4 *src = reinterpret_cast<const float4 *>(zrow + lo);
 #pragma unroll 4
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   Row r;
   r.s = min(50, 62 - (32 - __clz(n)));
   r.unit = __hiloint2double((1023 + r.s) << 20, 0);
-  r.c = fmax(46.166241308446828 / (double)T, 1e-300);  // 32 log2(e) / T
+  r.c = fmax(184.6649652337873 / (double)T, 1e-300);  // 128 log2(e) / T
   r.pow2 = sh.pow2;
   // below 2^-(s+2) of the maximum nothing counts
   r.cut = (r.s + 2) * 0.6931471805599453 * (double)T;
@@ -663,6 +664,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   const double u = fmin(fmax((double)u_row, 0.0), 1.0);
   cluster.sync();
   r.zmax = unordered(__reduce_max_sync(0xffffffffu, lane < C ? (uint32_t)cluster.map_shared_rank(&sh, lane)->best : 0u));
+  // (no infinity counts but as the maximum)
+  r.zcut = r.zmax == INFINITY ? INFINITY : fmaxf((float)((double)r.zmax - 1.01 * r.cut), -3.402823466e38f);
   const bool none = r.zmax == -INFINITY;
   if (none || !(T > 0.f)) {
     // nothing to draw, or the largest value: its last index
@@ -706,12 +709,15 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
       sh.mass = t;
     }
     cluster.sync();
-    u64 total = 0, before = 0;
-    for (int i = 0; i < C; ++i) {
-      const u64 x = cluster.map_shared_rank(&sh, i)->mass;
-      if (i < rank) before += x;
-      total += x;
+    // the CTAs' masses: all of them, and those of the CTAs before this one
+    u64 total = lane < C ? cluster.map_shared_rank(&sh, lane)->mass : 0, before = lane < rank ? total : 0;
+#pragma unroll
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
     }
+    total = __shfl_sync(0xffffffffu, total, 0);
+    before = __shfl_sync(0xffffffffu, before, 0);
     // the masses are read: the CTAs without the target leave while its one
     // goes on
     auto read = cluster.barrier_arrive();
@@ -850,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (in(z[j])) {
-              if (p < kList) boss_list[p] = (u64)ordered(z[j]) << 32 | (0xffffffffu - (uint32_t)(lo + i + j));
+              if (p < kList) boss_list[p] = (u64)ordered(z[j] + 0.f) << 32 | (0xffffffffu - (uint32_t)(lo + i + j));
               ++p;
             }
         });
