@@ -279,6 +279,14 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
   Book k = sh.book;
   int next = -1;
   constexpr int kPer = kBuckets / kThreads;
+  // the sum over the cluster's CTAs of what `get` reads
+  auto over = [&](auto get) {
+    const int lane = tid & 31;
+    u64 v = lane < C ? get(cluster.map_shared_rank(&sh, lane)) : 0;
+#pragma unroll
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+  };
   // first bucket that fulfils a condition that, once met, stays met
   auto find = [&](auto cond) {
     int mine = kBuckets;
@@ -300,23 +308,20 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
   int bk = kBuckets;  // the bucket in which the count reaches k_eff
   if (cmd == kHist) {
     // the cluster's counts, running sums in place, and the guessed masses
+    // (loads from another CTA take a microsecond: all of them at once)
     int c[kPer] = {};
     static_assert(kPer == 4, "");
+    int4 x[kMaxCluster];
+#pragma unroll
+    for (int q = 0; q < kMaxCluster; ++q) x[q] = reinterpret_cast<const int4 *>(cluster.map_shared_rank(hcount, min(q, C - 1)))[tid];
 #pragma unroll
     for (int q = 0; q < kMaxCluster; ++q)
-      if (q < C) {
-        const int4 x = reinterpret_cast<const int4 *>(cluster.map_shared_rank(hcount, q))[tid];
-        c[0] += x.x, c[1] += x.y, c[2] += x.z, c[3] += x.w;
-      }
-    if (level == 0 && masses) {
-      k.total = 0;
-      for (int q = 0; q < C; ++q) k.total += cluster.map_shared_rank(&sh, q)->mass;
-    }
+      if (q < C) c[0] += x[q].x, c[1] += x[q].y, c[2] += x[q].z, c[3] += x[q].w;
+    if (level == 0 && masses) k.total = over([](const Shared *p) { return p->mass; });
     if (first) {
       k.k_eff = t.top_k > 0 ? min(t.top_k, n) : n;
       if (t.min_p > 0.f) {
-        u64 above = 0;
-        for (int q = 0; q < C; ++q) above += cluster.map_shared_rank(&sh, q)->count;
+        const u64 above = over([](const Shared *p) { return (u64)p->count; });
         k.k_eff = min(k.k_eff, max(above, 1ull));
       }
     }
@@ -386,10 +391,14 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
     }
   } else if (cmd == kMass) {
     // ---- exact masses around the guess
-    u64 e = k.mup, mine = 0;
-    for (int q = 0; q < C; ++q) {
-      e += cluster.map_shared_rank(&sh, q)->mass;
-      if (tid < kWindow) mine += cluster.map_shared_rank(&sh, q)->window[tid];
+    const u64 e = k.mup + over([](const Shared *p) { return p->mass; });
+    u64 mine = 0;
+    if (tid < kWindow) {
+      u64 x[kMaxCluster];
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) x[q] = cluster.map_shared_rank(&sh, min(q, C - 1))->window[tid];
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) mine += q < C ? x[q] : 0;
     }
     const u64 front = e + block_before(mine, sh), back = front + mine;
     const u64 want = k.drawing ? k.target + 1 : k.p_mass;
@@ -440,21 +449,22 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
     // ---- sort what was gathered (falling value, rising index), running masses
     const int cnt = min(sh.listed, kList);
     u64 *sorted = list;
-    if (cnt <= kList / 2) {
-      // each thread counts the elements before its own (two at most), two a load
+    if (cnt <= kThreads) {
+      // each thread counts the elements before its own, two a load (at 512
+      // elements as long as the sort, and four times for twice as many)
       sorted = list + kList / 2;
       if (tid == 0 && (cnt & 1)) list[cnt] = 0;
       __syncthreads();
-      const u64 x = tid < cnt ? list[tid] : 0, y = tid + kThreads < cnt ? list[tid + kThreads] : 0;
-      int px = 0, py = 0;
+      if ((tid & ~31) < cnt) {
+        const u64 x = tid < cnt ? list[tid] : 0;
+        int px = 0;
 #pragma unroll 4
-      for (int i = 0; i < cnt; i += 2) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(list + i);
-        px += (q.x > x) + (q.y > x);
-        py += (q.x > y) + (q.y > y);
+        for (int i = 0; i < cnt; i += 2) {
+          const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(list + i);
+          px += (q.x > x) + (q.y > x);
+        }
+        if (tid < cnt) sorted[px] = x;
       }
-      if (tid < cnt) sorted[px] = x;
-      if (tid + kThreads < cnt) sorted[py] = y;
       __syncthreads();
     } else {
       int size = 2 * kThreads;
@@ -471,7 +481,7 @@ __device__ __noinline__ void leader_turn(Shared &sh, u64 *list, u64 *guess, int 
           __syncthreads();
         }
     }
-    const int each = cnt <= kThreads ? 1 : cnt <= kList / 2 ? 2 : kList / kThreads;
+    const int each = cnt <= kThreads ? 1 : cnt <= 2 * kThreads ? 2 : kList / kThreads;
     u64 m[kList / kThreads], ms = 0;
 #pragma unroll
     for (int j = 0; j < kList / kThreads; ++j) {
