@@ -19,7 +19,7 @@
 // cost about 20 instructions each, 11 of them in 64-bit floating point (an
 // SM does two warps' worth a clock), which overlap the reads of other rows.
 // One row alone is bound by latency: a cluster barrier takes 1 us. Measured:
-// one row of 32000 16 us; 64 rows of 128256 with all filters 99 us (0.33
+// one row of 32000 16 us; 64 rows of 128256 with all filters 94 us (0.35
 // TB/s of logits); 256 rows without a filter 103 us (1.28 TB/s).
 #include <cooperative_groups.h>
 
