@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
   __shared__ __align__(8) uint64_t raw_bar[2], s_bar, o_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ long long s_scan[kTcThreads / 32], s_tiles[kTcThreads / 32];
-  __shared__ float s_both[2][ROWS];  // what the two threads of a row exchange
+  __shared__ float s_both[2][ROWS], s_sum[2][ROWS];  // what the two threads of a row exchange: largest values, sums
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = tid & (ROWS - 1), half = tid / ROWS;
   if (tid == 0) {
@@ -563,9 +563,9 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
       add_output(1);
     }
     // ---- the segment's end, or the range's: the result, or a partial
-    s_both[half][row] = l;
+    s_sum[half][row] = l;
     __syncthreads();
-    const float sum = s_both[0][row] + s_both[1][row];
+    const float sum = s_sum[0][row] + s_sum[1][row];
     const bool whole = s.begin >= u0 && s.end <= u1;
     const float unit = kref == 1000 ? 0.f : __uint_as_float((uint32_t)max(0, 127 - 1 - kref) << 23);
     const float f = !whole ? unit : sum == 0.f ? 0.f : unit / sum;
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     }
     u = s.end;
     if (u < u1) {
-      __syncthreads();  // s_both is read
+      __syncthreads();  // the sums are read
       s = locate<ROWS>(a, pre, u);
     }
   }

@@ -183,6 +183,7 @@ def test_attention_chunks_whole_prompts_and_one_tile():
     check_attention([200, 129, 1, 64], [200, 129, 1, 64], 16, 8, 128)  # nothing cached before: each row sees up to itself
     check_attention([128], [128], 32, 8, 64)
     check_attention([64] * 12, [64] * 12, 8, 8, 64)  # a page a tile: no partial results
+    check_attention([70 + 9 * i for i in range(32)], [1] * 32, 64, 1, 128)  # many heads on one, a row per sequence
 
 
 def test_attention_chunks_streams_and_graph():
