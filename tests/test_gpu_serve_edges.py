@@ -1,0 +1,98 @@
+"""Edges of the paged serving step's operators, against serve_rule.py's 64-bit
+restatements: values of very different sizes under the attention's sums."""
+import numpy as np
+import pytest
+import torch
+
+import serve_rule as SR
+from inferox_b200 import ops
+from test_gpu_serve_ops import cuda, filled, i32
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def store(pages, table, b, k, v):
+    """Rows k, v of sequence b into its pages; the values they then stand for."""
+    t = np.arange(len(k))
+    k, v = np.asarray(k, np.float32), np.asarray(v, np.float32)
+    ops.kv4_store(cuda(k), cuda(v), i32(table[b, t // 64] * 64 + t % 64), pages)
+    return SR.values(*SR.quantise(k)), SR.values(*SR.quantise(v))
+
+
+def own_bound(q, K, V, lens, start, scale, window=0):
+    """The result in 64 bits, and a bound from what each row sees itself: a
+    score's error as in test_gpu_serve_ops.bound, and twice that of a
+    probability; 2^-20 for the exponential and the planes of 22 bits; per
+    page of 64 rows fixed-point steps of 2^-21 (half of 4 / 4.1e6) of the
+    largest term, eight deviations of 64 of them, which f32's own sums stay
+    below; relative to the magnitudes summed, at their largest in a block of
+    32 dimensions (its largest value is what a block's scale is made for)."""
+    ref, worst = SR.attention(q, K, V, lens, start, scale, window)
+    mag = SR.attention(q, K, [np.abs(v) for v in V], lens, start, scale, window)[0]
+    mag = np.repeat(mag.reshape(*mag.shape[:-1], -1, 32).max(-1), 32, -1)
+    n, hd = max(lens), q.shape[-1]
+    rel = 2 * (hd + 16) * 2.0 ** -24 * worst + 2.0 ** -20 + 8 * 8 * 2.0 ** -21 / 3 ** 0.5 + 8 * np.sqrt(n + 1) * 2.0 ** -24
+    return ref, mag * rel + np.abs(ref) * 2.0 ** -24
+
+
+def close(got, ref, lim):
+    err = np.abs(got.float().cpu().numpy().astype(np.float64) - ref)
+    assert np.all(err <= lim), (float(err.max()), float((err / np.maximum(lim, 1e-300)).max()))
+
+
+def spread(rng, n, G, hd, scores):
+    """Keys whose product with a query of 1 in dimension 0 is scores [n], and a little of the rest."""
+    k = 0.01 * rng.standard_normal((n, G, hd))
+    k[..., :32] = 0
+    k[..., 0] = np.float16(np.asarray(scores) / 8)[:, None].astype(np.float64) * 8
+    return k
+
+
+def ones_first(rng, rows, H, hd):
+    q = 0.1 * rng.standard_normal((rows, H, hd)).astype(np.float32)
+    q[..., 0] = 1
+    return q
+
+
+@pytest.mark.parametrize("H,G,hd", [(32, 8, 64), (8, 4, 128), (8, 4, 256)])
+@pytest.mark.parametrize("ql", [1, 6, 128])
+@pytest.mark.parametrize("after", [1, 5, 20, 60])
+def test_attention_pages_of_zero_values(H, G, hd, ql, after):
+    """One key that stands out, then pages whose values are all 0 with scores 8
+    to 12 powers of two below it: they weigh in the sum of every row."""
+    rng = np.random.default_rng(after)
+    n, seqs = 64 * (1 + after) + ql, 2
+    pages, table, K, V = filled(rng, [n] * seqs, G, hd)
+    for b in range(seqs):
+        s = -np.log(2) * rng.uniform(8, 12, n)
+        s[3] = 0
+        v = rng.standard_normal((n, G, hd))
+        v[64:64 * (1 + after)] = 0
+        K[b], V[b] = store(pages, table, b, spread(rng, n, G, hd, s), v)
+    q, start = ones_first(rng, seqs * ql, H, hd), ql * np.arange(seqs + 1)
+    ref, lim = own_bound(q, K, V, [n] * seqs, start, 1.0)
+    close(ops.kv4_attention(cuda(q), pages, i32(table), i32([n] * seqs), G, q_start=i32(start), scale=1.0), ref, lim)
+
+
+@pytest.mark.parametrize("H,G,hd", [(32, 8, 64), (8, 4, 128), (8, 4, 256)])
+@pytest.mark.parametrize("ql", [1, 6, 128])
+@pytest.mark.parametrize("big_first", [True, False])
+@pytest.mark.parametrize("low", [3e-6, 1e-3, 1.0, 100.0])
+def test_attention_pages_of_unequal_values(H, G, hd, ql, big_first, low):
+    """A page of large values that hardly weighs beside pages of small ones
+    that carry the weight, before them and behind them."""
+    rng = np.random.default_rng(int(low * 1e6) + big_first)
+    n, seqs = 64 * 5 + ql, 2
+    at = 0 if big_first else 192
+    pages, table, K, V = filled(rng, [n] * seqs, G, hd)
+    for b in range(seqs):
+        s = rng.uniform(-2, 0, n)
+        s[at:at + 64] -= 40
+        v = low * rng.standard_normal((n, G, hd))
+        v[at:at + 64] = 50000 * rng.uniform(-1, 1, (64, G, hd))
+        K[b], V[b] = store(pages, table, b, spread(rng, n, G, hd, s), v)
+    q, start = ones_first(rng, seqs * ql, H, hd), ql * np.arange(seqs + 1)
+    ref, lim = own_bound(q, K, V, [n] * seqs, start, 1.0)
+    close(ops.kv4_attention(cuda(q), pages, i32(table), i32([n] * seqs), G, q_start=i32(start), scale=1.0), ref, lim)
