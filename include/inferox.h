@@ -262,9 +262,12 @@ ifx_status ifx_sample(ifx_model *m, const ifx_sampler *s, uint64_t seed,
 
 /* Sampler::sample's rule (sampler.rs:28-73) for rows 0 .. n-1 of the latest
  * logits on the device: those of kb's latest decode step (row i is the
- * caller's row i), or of its latest prompt's last row (n = 1); kb NULL: the
- * model's latest logits (n = 1). Each row has its own settings s[i], min_p[i]
- * (nullable: none) and draw u[i] in [0, 1), as ifx_op_sample_rows describes.
+ * caller's row i), or of its latest prompt's last row (n = 1), whatever other
+ * caches of the model have done since; kb NULL: the model's latest logits
+ * (n = 1). A call that was refused (a bad token, a dry pool) leaves the rows of
+ * the one before; after one that failed on its way there are none. Each row
+ * has its own settings s[i], min_p[i] (nullable: none) and draw u[i] in
+ * [0, 1), as ifx_op_sample_rows describes.
  * tokens [n] (0xffffffff where every logit is masked); logprobs [n] is
  * nullable. Host buffers; returns when the tokens are there. */
 ifx_status ifx_sample_batch(ifx_model *m, ifx_kv_batch *kb, int n,

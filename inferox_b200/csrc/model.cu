@@ -747,12 +747,6 @@ ifx_status KvBatch::reserve(int seq, size_t rows, cudaStream_t st) {
   return IFX_OK;
 }
 
-void KvBatch::latest_rows(int n) {
-  order.resize((size_t)n);
-  for (int i = 0; i < n; ++i) order[(size_t)i] = i;
-  after_prompt = false;
-}
-
 void KvBatch::release(int seq) {
   if (!paged) return;
   int *row = table.data() + (size_t)seq * max_pages;
@@ -1152,11 +1146,11 @@ ifx_status Model::prefill_seq(KvBatch &kb, int seq, const uint32_t *ids, size_t 
   view.m = this;
   view.max_seq = kb.max_seq;
   view.per_layer = kb.per_layer;
+  for (size_t i = 0; i < n; ++i)
+    if (ids[i] >= cfg.vocab_size) return fail(IFX_ERR_INVALID_TENSOR_INDEX, "tensor index out of bounds: 0");
+  if (n == 0) return IFX_OK;
   std::vector<int> add;
   if (kb.q4) {
-    for (size_t i = 0; i < n; ++i)
-      if (ids[i] >= cfg.vocab_size) return fail(IFX_ERR_INVALID_TENSOR_INDEX, "tensor index out of bounds: 0");
-    if (n == 0) return IFX_OK;
     IFX_CUDA(cudaSetDevice(device));
     IFX_TRY(ensure_ws(n));
     IFX_TRY(kb.take(&seq, 1, n));
@@ -1176,17 +1170,22 @@ ifx_status Model::prefill_seq(KvBatch &kb, int seq, const uint32_t *ids, size_t 
     view.page_rows = kb.page_rows;
     view.page_stride = kb.page_stride;
   } else {
+    if (kb.len[(size_t)seq] + n > kb.max_seq)
+      return fail(IFX_ERR_INVALID_TENSOR_INDEX, "prompt exceeds the KV cache");
     view.k = kb.k + (size_t)seq * cfg.n_layers * kb.per_layer;
     view.v = kb.v + (size_t)seq * cfg.n_layers * kb.per_layer;
   }
   view.pos = kb.pos + seq;
   view.len = kb.len[(size_t)seq];
   view.mega_tried = true;  // never planned for the persistent kernel
+  kb.order.clear();
   const ifx_status s = run_prompt(&view, ids, n, logits_host, last_row_only);
-  kb.order.assign(1, 0);
-  kb.after_prompt = true;
   kb.len[(size_t)seq] = view.len;
-  return s;
+  if (s != IFX_OK) return s;
+  // sampling draws from the batch's own rows: the model's buffer is the next call's
+  IFX_CUDA(cudaMemcpyAsync(kb.logits, logits, sizeof(float) * cfg.vocab_size, cudaMemcpyDeviceToDevice, stream));
+  kb.order.assign(1, 0);
+  return IFX_OK;
 }
 
 // One decode step of every sequence of the batch (Model::decode_step,
@@ -1304,6 +1303,12 @@ ifx_status Model::enqueue_decode_batch(KvBatch &kb, cudaStream_t st, int n, cons
   return IFX_OK;
 }
 
+static std::vector<int> rows_in_order(int n) {
+  std::vector<int> rows((size_t)n);
+  for (int i = 0; i < n; ++i) rows[(size_t)i] = i;
+  return rows;
+}
+
 ifx_status Model::decode_batch(KvBatch &kb, const uint32_t *tokens, float *logits_host,
                                uint32_t *argmax_host) {
   NvtxRange nvtx_("ifx:decode_step_batch");
@@ -1318,7 +1323,7 @@ ifx_status Model::decode_batch(KvBatch &kb, const uint32_t *tokens, float *logit
   if (kb.q4) IFX_TRY(kb.take(nullptr, kb.batch, 1));
   for (int b = 0; b < kb.batch; ++b) IFX_TRY(kb.reserve(b, kb.len[(size_t)b] + 1, st));
   IFX_CUDA(cudaMemcpyAsync(kb.ids, tokens, sizeof(uint32_t) * kb.batch, cudaMemcpyHostToDevice, st));
-  kb.latest_rows(kb.batch);
+  kb.order.clear();
   IFX_TRY(enqueue_decode_batch(kb, st));
   if (logits_host)
     IFX_CUDA(cudaMemcpyAsync(logits_host, kb.logits, sizeof(float) * kb.batch * cfg.vocab_size,
@@ -1328,7 +1333,9 @@ ifx_status Model::decode_batch(KvBatch &kb, const uint32_t *tokens, float *logit
                              cudaMemcpyDeviceToHost, st));
   IFX_CUDA(cudaStreamSynchronize(st));
   for (auto &n : kb.len) n += 1;
-  return check_err();
+  IFX_TRY(check_err());
+  kb.order = rows_in_order(kb.batch);
+  return IFX_OK;
 }
 
 // One decode step of the n distinct sequences seqs[0..n) of the batch (a
@@ -1350,7 +1357,7 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
   }
   IFX_CUDA(cudaSetDevice(device));
   cudaStream_t st = stream;
-  kb.latest_rows(n);
+  std::vector<int> order = rows_in_order(n);  // the caller's row i is row order[i] of the step
   std::vector<int> sorted_seqs, add;
   std::vector<uint32_t> sorted_tokens, sorted_out;
   if (kb.q4) {
@@ -1364,7 +1371,7 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
     for (int i = 0; i < n; ++i) {
       sorted_seqs.push_back(seqs[at[(size_t)i]]);
       sorted_tokens.push_back(tokens[at[(size_t)i]]);
-      kb.order[(size_t)at[(size_t)i]] = i;
+      order[(size_t)at[(size_t)i]] = i;
       add[(size_t)seqs[i]] = 1;
     }
     IFX_CUDA(cudaMemcpyAsync(kb.add4, add.data(), sizeof(int) * kb.batch, cudaMemcpyHostToDevice, st));
@@ -1374,22 +1381,25 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
   for (int i = 0; i < n; ++i) IFX_TRY(kb.reserve(seqs[i], kb.len[(size_t)seqs[i]] + 1, st));
   IFX_CUDA(cudaMemcpyAsync(kb.ids, run_tokens, sizeof(uint32_t) * n, cudaMemcpyHostToDevice, st));
   IFX_CUDA(cudaMemcpyAsync(kb.slots, run_seqs, sizeof(int) * n, cudaMemcpyHostToDevice, st));
+  kb.order.clear();
   IFX_TRY(enqueue_decode_batch(kb, st, n, kb.slots));
   if (logits_host && !kb.q4)
     IFX_CUDA(cudaMemcpyAsync(logits_host, kb.logits, sizeof(float) * n * cfg.vocab_size,
                              cudaMemcpyDeviceToHost, st));
   for (int i = 0; logits_host && kb.q4 && i < n; ++i)
     IFX_CUDA(cudaMemcpyAsync(logits_host + (size_t)i * cfg.vocab_size,
-                             kb.logits + (size_t)kb.order[(size_t)i] * cfg.vocab_size,
+                             kb.logits + (size_t)order[(size_t)i] * cfg.vocab_size,
                              sizeof(float) * cfg.vocab_size, cudaMemcpyDeviceToHost, st));
   if (argmax_host) {
     sorted_out.resize((size_t)n);
     IFX_CUDA(cudaMemcpyAsync(sorted_out.data(), kb.out, sizeof(uint32_t) * n, cudaMemcpyDeviceToHost, st));
   }
   IFX_CUDA(cudaStreamSynchronize(st));
-  for (int i = 0; argmax_host && i < n; ++i) argmax_host[i] = sorted_out[(size_t)kb.order[(size_t)i]];
+  for (int i = 0; argmax_host && i < n; ++i) argmax_host[i] = sorted_out[(size_t)order[(size_t)i]];
   for (int i = 0; i < n; ++i) kb.len[(size_t)seqs[i]] += 1;
-  return check_err();
+  IFX_TRY(check_err());
+  kb.order = std::move(order);
+  return IFX_OK;
 }
 
 // Draws for rows 0..n-1 of the latest logits: row-wise sampling (op_sample_rows)
@@ -1397,9 +1407,8 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
 ifx_status Model::sample_batch(KvBatch *kb, int n, const ifx_sampler *s, const float *min_p, const float *u,
                                uint32_t *tokens, float *logprobs) {
   NvtxRange nvtx_("ifx:sample_batch");
-  const bool of_model = !kb || kb->after_prompt;
   const int rows = kb ? (int)kb->order.size() : 1;
-  if (n < 1 || n > (of_model ? 1 : rows))
+  if (n < 1 || n > rows)
     return fail(IFX_ERR_INVALID_ARGUMENT, "sample_batch: no such row in the latest logits");
   IFX_CUDA(cudaSetDevice(device));
   constexpr int W = 7;  // u, temperature, top_k, top_p, min_p; token, logprob
@@ -1408,7 +1417,7 @@ ifx_status Model::sample_batch(KvBatch *kb, int n, const ifx_sampler *s, const f
   std::vector<float> in((size_t)5 * rows, 0.f), out((size_t)2 * rows);
   for (int r = 0; r < rows; ++r) in[(size_t)(3 * rows + r)] = 1.f;  // rows not asked for: greedy
   for (int i = 0; i < n; ++i) {
-    const int r = of_model ? 0 : kb->order[(size_t)i];
+    const int r = kb ? kb->order[(size_t)i] : 0;
     const int k = (int)std::min<uint64_t>(s[i].top_k, (uint64_t)INT32_MAX);
     in[(size_t)r] = u[i];
     in[(size_t)(rows + r)] = s[i].temperature;
@@ -1419,13 +1428,13 @@ ifx_status Model::sample_batch(KvBatch *kb, int n, const ifx_sampler *s, const f
   IFX_CUDA(cudaMemcpyAsync(sample_buf, in.data(), in.size() * sizeof(float), cudaMemcpyHostToDevice, st));
   float *b = sample_buf, *o = b + (size_t)5 * rows;
   const int64_t V = (int64_t)cfg.vocab_size;
-  SampleRowsArgs a{of_model ? logits : kb->logits, rows, V, V, b, b + rows, reinterpret_cast<int *>(b + 2 * rows),
+  SampleRowsArgs a{kb ? kb->logits : logits, rows, V, V, b, b + rows, reinterpret_cast<int *>(b + 2 * rows),
                    b + 3 * rows, b + 4 * rows, reinterpret_cast<int *>(o), o + rows};
   IFX_TRY(op_sample_rows(a, st));
   IFX_CUDA(cudaMemcpyAsync(out.data(), o, out.size() * sizeof(float), cudaMemcpyDeviceToHost, st));
   IFX_TRY(step_sync(st));
   for (int i = 0; i < n; ++i) {
-    const int r = of_model ? 0 : kb->order[(size_t)i];
+    const int r = kb ? kb->order[(size_t)i] : 0;
     memcpy(&tokens[i], &out[(size_t)r], sizeof(uint32_t));
     if (logprobs) logprobs[i] = out[(size_t)(rows + r)];
   }
@@ -1520,7 +1529,6 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
   cudaStream_t st = stream;
   if (kb.q4) IFX_TRY(kb.take(nullptr, kb.batch, n));
   for (int b = 0; b < kb.batch; ++b) IFX_TRY(kb.reserve(b, kb.len[(size_t)b] + n, st));
-  if (n) kb.latest_rows(kb.batch);
   uint32_t *toks = nullptr;  // every step's tokens, copied out once at the end
   IFX_TRY(dalloc(&toks, std::max<size_t>(1, n) * kb.batch));
   IFX_CUDA(cudaMemcpyAsync(kb.ids, tokens, sizeof(uint32_t) * kb.batch, cudaMemcpyHostToDevice, st));
@@ -1531,6 +1539,7 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
     IFX_CUDA(cudaEventRecord(e0, st));
   }
   ifx_status s = IFX_OK;
+  if (n) kb.order.clear();
   for (size_t i = 0; i < n && s == IFX_OK; ++i) {
     s = step_batch_fed(kb, st);
     if (s == IFX_OK)
@@ -1549,7 +1558,9 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
   }
   IFX_TRY(s);
   for (auto &l : kb.len) l += n;
-  return check_err();
+  IFX_TRY(check_err());
+  if (n) kb.order = rows_in_order(kb.batch);
+  return IFX_OK;
 }
 
 // Shared body of prefill (kvp set: causal attention, K/V appended to the

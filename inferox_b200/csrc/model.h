@@ -108,11 +108,10 @@ struct KvBatch {
   // with no change when there are too few
   ifx_status take(const int *seqs, int n, size_t rows);
   ifx_status extend(const int *add, size_t max_tokens, cudaStream_t st);
-  // the rows that sampling draws from: those of the latest step (caller's row
-  // i at order[i]), or the latest prompt's last one
+  // the rows of `logits` that sampling draws from: those of the latest step
+  // (caller's row i at order[i]), or the latest prompt's last one; empty where
+  // there are none, after a call that failed on its way too
   std::vector<int> order;
-  bool after_prompt = false;
-  void latest_rows(int n);
   ifx_status create(Model *model, size_t max_seq_len, int nseq, size_t pages = 0);
   // give sequence `seq` pages for positions [0, rows); fails with no change
   // when the pool runs out
