@@ -41,6 +41,7 @@ ifx_status fail(ifx_status s, const std::string &msg) {
 
 ifx_status cuda_fail(cudaError_t e, const char *what) {
   g_last_error = std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")";
+  cudaGetLastError();  // reported here, not to the next call's launches
   if (e == cudaErrorMemoryAllocation) return IFX_ERR_OUT_OF_MEMORY;
   return IFX_ERR_CUDA;
 }

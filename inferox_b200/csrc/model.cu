@@ -1094,6 +1094,7 @@ ifx_status Model::ensure_ws(size_t n) {
   if (ids_dev) cudaFree(ids_dev);
   ws = nullptr;
   ids_dev = nullptr;
+  ws_tokens = 0;  // nothing is there until both allocations have succeeded
   const ifx_config &c = cfg;
   const size_t D = c.hidden_size, Hh = Hl * c.head_dim, kvd = Gl * c.head_dim;
   const size_t F = Fl;
@@ -1563,6 +1564,17 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
   return IFX_OK;
 }
 
+// A buffer of at least n floats; none, and size 0, where there is no memory.
+static ifx_status grow(float **p, size_t *have, size_t n) {
+  if (n <= *have) return IFX_OK;
+  if (*p) cudaFree(*p);
+  *p = nullptr;
+  *have = 0;
+  IFX_CUDA(cudaMalloc(p, n * sizeof(float)));
+  *have = n;
+  return IFX_OK;
+}
+
 // Shared body of prefill (kvp set: causal attention, K/V appended to the
 // cache) and forward (kvp null: full attention, no cache).
 ifx_status Model::run_prompt(KvCache *kvp, const uint32_t *ids, size_t n, float *logits_host,
@@ -1578,6 +1590,11 @@ ifx_status Model::run_prompt(KvCache *kvp, const uint32_t *ids, size_t n, float 
     return fail(IFX_ERR_INVALID_TENSOR_INDEX, "prompt exceeds the KV cache");
   IFX_CUDA(cudaSetDevice(device));
   IFX_TRY(ensure_ws(n));
+  // memory first: a call that does not get it changes nothing
+  if (!last_row_only && logits_host) {
+    IFX_TRY(grow(&logits_all, &logits_all_n, n * c.vocab_size));
+    if (tp > 1) IFX_TRY(grow(&logits_all_local, &logits_all_local_n, 2 * n * Vl * tp));
+  }
   cudaStream_t st = stream;
   const int64_t N = (int64_t)n;
   const int D = (int)c.hidden_size, H = (int)Hl, G = (int)Gl, hd = (int)c.head_dim;
@@ -1673,22 +1690,10 @@ ifx_status Model::run_prompt(KvCache *kvp, const uint32_t *ids, size_t n, float 
                                cudaMemcpyDeviceToHost, st));
   } else {
     const size_t need = n * c.vocab_size;
-    if (need > logits_all_n) {
-      if (logits_all) cudaFree(logits_all);
-      logits_all = nullptr;
-      IFX_CUDA(cudaMalloc(&logits_all, need * sizeof(float)));
-      logits_all_n = need;
-    }
     IFX_TRY(stage_rows(w_x, nullptr, out_norm, c.norm_eps, GX_RMSNORM, N, D, w_xf, st));
     if (tp > 1) {
       // [n][Vl] per rank, gathered rank-major, then interleaved to [n][V]
       const size_t loc = n * Vl;
-      if (2 * loc * tp > logits_all_local_n) {
-        if (logits_all_local) cudaFree(logits_all_local);
-        logits_all_local = nullptr;
-        IFX_CUDA(cudaMalloc(&logits_all_local, 2 * loc * tp * sizeof(float)));
-        logits_all_local_n = 2 * loc * tp;
-      }
       float *mine = logits_all_local, *gathered = logits_all_local + loc * tp;
       IFX_TRY(gemm_run(out_w, w_xf, N, mine, (int)Vl, 0, err, st));
       IFX_NCCL(nccl, nccl->AllGather(mine, gathered, loc, ncclFloat32, (ncclComm_t)comm, st));
