@@ -208,7 +208,8 @@ ifx_status ifx_kv_batch_create_paged(ifx_model *m, size_t max_seq_len, int batch
  * as they are stored, so decode steps see the quantised rows; attention
  * within a prompt uses its rows as computed. head_dim 32, 64, 96 or 128; no
  * bound on max_seq_len but the pool. Otherwise as
- * ifx_kv_batch_create_paged. */
+ * ifx_kv_batch_create_paged; a call on it that fails on its way drops the
+ * rows it brought and gives their pages back. */
 ifx_status ifx_kv_batch_create_q4(ifx_model *m, size_t max_seq_len, int batch,
                                   size_t n_pages, ifx_kv_batch **out);
 /* Pages of a paged batch that no sequence holds, and the pool size (both 0

@@ -135,6 +135,14 @@ __global__ void kv_write_paged_kernel(const float *k, const float *v, __half *kc
 
 __global__ void add_int_kernel(int *p, int v) { *p += v; }
 
+// The free list's new length, and an error where the tables refused the step's
+// rows: the host counts pages too, and the two have to agree.
+constexpr int kErrPages = 501;
+__global__ void pages_taken_kernel(const int *n_free_new, const int *status, int *n_free, int *err) {
+  *n_free = *n_free_new;
+  if (*status) atomicExch(err, kErrPages);
+}
+
 // Row-wise argmax of x [rows][n] (last index on ties, NaN skipped:
 // forward.rs:615-622): CTA (row, part) reduces a contiguous part of the row
 // to a 64-bit key (ordered value bits << 32 | index) and takes the maximum
@@ -712,9 +720,58 @@ ifx_status KvBatch::extend(const int *add, size_t max_tokens, cudaStream_t st) {
   PagesExtendArgs e{pos, add, batch, table_dev, max_pages, free4, (int)n_pages, n_free4, (int64_t)max_tokens,
                     lens4, nf, qs, slots4, positions4, nullptr, status};
   IFX_TRY(op_pages_extend(e, st));
-  IFX_CUDA(cudaMemcpyAsync(n_free4, nf, sizeof(int), cudaMemcpyDeviceToDevice, st));
+  pages_taken_kernel<<<1, 1, 0, st>>>(nf, status, n_free4, m->err);
+  IFX_CUDA(cudaGetLastError());
   return IFX_OK;
 }
+
+// After a call that failed on its way: lengths, table and free list on the
+// device, and the counts here, as `len` has them. The pages that rows below it
+// lie in have not moved (op_pages_extend writes table entries above them only).
+void KvBatch::recover(cudaStream_t st) noexcept try {
+  std::vector<int> rows((size_t)batch * max_pages), lens((size_t)batch), list;
+  std::vector<char> used(n_pages, 0);
+  if (cudaStreamSynchronize(st) != cudaSuccess ||
+      cudaMemcpyAsync(rows.data(), table_dev, rows.size() * sizeof(int), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      cudaStreamSynchronize(st) != cudaSuccess)
+    return;  // nothing works any more
+  n_free = n_pages;
+  for (int b = 0; b < batch; ++b) {
+    lens[(size_t)b] = (int)len[(size_t)b];
+    held[(size_t)b] = (int)((len[(size_t)b] + page_rows - 1) / page_rows);
+    n_free -= (size_t)held[(size_t)b];
+    for (int j = 0; j < held[(size_t)b]; ++j) {
+      const int page = rows[(size_t)b * max_pages + j];
+      if (page >= 0 && (size_t)page < n_pages) used[(size_t)page] = 1;
+    }
+  }
+  for (size_t i = n_pages; i-- > 0;)
+    if (!used[i]) list.push_back((int)i);
+  const int n = (int)n_free;
+  cudaMemcpyAsync(free4, list.data(), list.size() * sizeof(int), cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(n_free4, &n, sizeof(int), cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(pos, lens.data(), lens.size() * sizeof(int), cudaMemcpyHostToDevice, st);
+  cudaStreamSynchronize(st);
+} catch (...) {
+}
+
+namespace {
+// A call that takes pages: what it took goes back unless it is done.
+struct PagesGuard {
+  KvBatch &kb;
+  cudaStream_t st;
+  bool armed = false;
+  ~PagesGuard() {
+    if (armed) kb.recover(st);
+  }
+  ifx_status take(const int *seqs, int n, size_t rows) {
+    if (!kb.q4) return IFX_OK;
+    IFX_TRY(kb.take(seqs, n, rows));
+    armed = true;
+    return IFX_OK;
+  }
+};
+}  // namespace
 
 KvBatch::~KvBatch() {
   if (dev >= 0) cudaSetDevice(dev);
@@ -1064,6 +1121,7 @@ ifx_status Model::check_err() {
     // stopped (the persistent kernel's all-reduce epochs, the collectives):
     // refuse further calls, as after an aborted communicator
     if (tp > 1) comm_aborted = true;
+    if (h == kErrPages) return fail(IFX_ERR_CUDA, "4-bit cache: the page tables refused rows that the host had counted");
     return fail(IFX_ERR_TIMEOUT, "a bounded device wait gave up (code " + std::to_string(h) + ")");
   }
   return IFX_OK;
@@ -1151,10 +1209,11 @@ ifx_status Model::prefill_seq(KvBatch &kb, int seq, const uint32_t *ids, size_t 
     if (ids[i] >= cfg.vocab_size) return fail(IFX_ERR_INVALID_TENSOR_INDEX, "tensor index out of bounds: 0");
   if (n == 0) return IFX_OK;
   std::vector<int> add;
+  PagesGuard guard{kb, stream};
   if (kb.q4) {
     IFX_CUDA(cudaSetDevice(device));
     IFX_TRY(ensure_ws(n));
-    IFX_TRY(kb.take(&seq, 1, n));
+    IFX_TRY(guard.take(&seq, 1, n));
     add.assign((size_t)kb.batch, 0);
     add[(size_t)seq] = (int)n;
     IFX_CUDA(cudaMemcpyAsync(kb.add4, add.data(), sizeof(int) * kb.batch, cudaMemcpyHostToDevice, stream));
@@ -1181,8 +1240,9 @@ ifx_status Model::prefill_seq(KvBatch &kb, int seq, const uint32_t *ids, size_t 
   view.mega_tried = true;  // never planned for the persistent kernel
   kb.order.clear();
   const ifx_status s = run_prompt(&view, ids, n, logits_host, last_row_only);
-  kb.len[(size_t)seq] = view.len;
+  if (s == IFX_OK || !kb.q4) kb.len[(size_t)seq] = view.len;
   if (s != IFX_OK) return s;
+  guard.armed = false;
   // sampling draws from the batch's own rows: the model's buffer is the next call's
   IFX_CUDA(cudaMemcpyAsync(kb.logits, logits, sizeof(float) * cfg.vocab_size, cudaMemcpyDeviceToDevice, stream));
   kb.order.assign(1, 0);
@@ -1321,7 +1381,8 @@ ifx_status Model::decode_batch(KvBatch &kb, const uint32_t *tokens, float *logit
   }
   IFX_CUDA(cudaSetDevice(device));
   cudaStream_t st = stream;
-  if (kb.q4) IFX_TRY(kb.take(nullptr, kb.batch, 1));
+  PagesGuard guard{kb, st};
+  IFX_TRY(guard.take(nullptr, kb.batch, 1));
   for (int b = 0; b < kb.batch; ++b) IFX_TRY(kb.reserve(b, kb.len[(size_t)b] + 1, st));
   IFX_CUDA(cudaMemcpyAsync(kb.ids, tokens, sizeof(uint32_t) * kb.batch, cudaMemcpyHostToDevice, st));
   kb.order.clear();
@@ -1333,8 +1394,11 @@ ifx_status Model::decode_batch(KvBatch &kb, const uint32_t *tokens, float *logit
     IFX_CUDA(cudaMemcpyAsync(argmax_host, kb.out, sizeof(uint32_t) * kb.batch,
                              cudaMemcpyDeviceToHost, st));
   IFX_CUDA(cudaStreamSynchronize(st));
-  for (auto &n : kb.len) n += 1;
-  IFX_TRY(check_err());
+  const ifx_status s = check_err();
+  if (s == IFX_OK || !kb.q4)
+    for (auto &n : kb.len) n += 1;
+  IFX_TRY(s);
+  guard.armed = false;
   kb.order = rows_in_order(kb.batch);
   return IFX_OK;
 }
@@ -1361,10 +1425,11 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
   std::vector<int> order = rows_in_order(n);  // the caller's row i is row order[i] of the step
   std::vector<int> sorted_seqs, add;
   std::vector<uint32_t> sorted_tokens, sorted_out;
+  PagesGuard guard{kb, st};
+  IFX_TRY(guard.take(seqs, n, 1));
   if (kb.q4) {
     // the device lays rows out by sequence: the step runs in that order, and
     // row i of the results is put back to seqs[i]
-    IFX_TRY(kb.take(seqs, n, 1));
     std::vector<int> at((size_t)n);
     for (int i = 0; i < n; ++i) at[(size_t)i] = i;
     std::sort(at.begin(), at.end(), [&](int x, int y) { return seqs[x] < seqs[y]; });
@@ -1397,8 +1462,11 @@ ifx_status Model::decode_batch_seqs(KvBatch &kb, const int *seqs, int n, const u
   }
   IFX_CUDA(cudaStreamSynchronize(st));
   for (int i = 0; argmax_host && i < n; ++i) argmax_host[i] = sorted_out[(size_t)order[(size_t)i]];
-  for (int i = 0; i < n; ++i) kb.len[(size_t)seqs[i]] += 1;
-  IFX_TRY(check_err());
+  const ifx_status s = check_err();
+  if (s == IFX_OK || !kb.q4)
+    for (int i = 0; i < n; ++i) kb.len[(size_t)seqs[i]] += 1;
+  IFX_TRY(s);
+  guard.armed = false;
   kb.order = std::move(order);
   return IFX_OK;
 }
@@ -1528,7 +1596,8 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
   }
   IFX_CUDA(cudaSetDevice(device));
   cudaStream_t st = stream;
-  if (kb.q4) IFX_TRY(kb.take(nullptr, kb.batch, n));
+  PagesGuard guard{kb, st};
+  IFX_TRY(guard.take(nullptr, kb.batch, n));
   for (int b = 0; b < kb.batch; ++b) IFX_TRY(kb.reserve(b, kb.len[(size_t)b] + n, st));
   uint32_t *toks = nullptr;  // every step's tokens, copied out once at the end
   IFX_TRY(dalloc(&toks, std::max<size_t>(1, n) * kb.batch));
@@ -1558,8 +1627,10 @@ ifx_status Model::decode_greedy_batch(KvBatch &kb, const uint32_t *tokens, size_
     cudaEventDestroy(e1);
   }
   IFX_TRY(s);
+  if (kb.q4) IFX_TRY(check_err());
   for (auto &l : kb.len) l += n;
   IFX_TRY(check_err());
+  guard.armed = false;
   if (n) kb.order = rows_in_order(kb.batch);
   return IFX_OK;
 }

@@ -108,6 +108,7 @@ struct KvBatch {
   // with no change when there are too few
   ifx_status take(const int *seqs, int n, size_t rows);
   ifx_status extend(const int *add, size_t max_tokens, cudaStream_t st);
+  void recover(cudaStream_t st) noexcept;
   // the rows of `logits` that sampling draws from: those of the latest step
   // (caller's row i at order[i]), or the latest prompt's last one; empty where
   // there are none, after a call that failed on its way too

@@ -68,3 +68,28 @@ def check(kind, full_device):
 @pytest.mark.parametrize("kind", ["cache", "batch", "paged"])
 def test_prompt_without_memory_changes_nothing(kind, full_device):
     check(kind, full_device)
+
+
+def test_prompt_without_memory_gives_its_pages_back(full_device):
+    """The cache in 4 bits: the tables on the device had taken the prompt's
+    pages when the call failed. Every page of the pool is there afterwards."""
+    check("q4", full_device)
+    m, ids = _model(), synth.prompt_ids(V, N, seed=1)
+    kb = m.kv_batch(3, 4096, 70, 4)
+    for s in (0, 1):
+        kb.prefill(s, ids[:100 + 800 * s], True)  # two pages and fifteen
+    kb.prefill(2, ids, True)
+    kb.reset(2)
+    assert kb.pages() == (53, 70)
+    for _ in range(3):
+        with pytest.raises(IfxError, match="OutOfMemory"):
+            full_device(lambda: kb.prefill(2, ids, False))
+        assert kb.pages() == (53, 70) and [kb.len(s) for s in range(3)] == [100, 900, 0]
+    kb.prefill(2, synth.prompt_ids(V, 53 * 64, seed=2), True)  # the last page
+    assert kb.pages() == (0, 70)
+    logits = kb.decode_step_seqs([0, 1], [5, 6])[0]
+    kb = m.kv_batch(3, 4096, 70, 4)
+    for s in (0, 1):
+        kb.prefill(s, ids[:100 + 800 * s], True)
+    want = kb.decode_step_seqs([0, 1], [5, 6])[0]
+    assert np.all(np.abs(logits - want) <= 4 * 512 * 2.0 ** -24 * 10), float(np.abs(logits - want).max())
