@@ -12,7 +12,9 @@ maxima, forward.rs:615-622), then the argmax after feeding each token back.
 A request submitted with a `sampler` (and a `seed`) draws its tokens instead:
 token i is drawn from its row's logits with the uniform number of (seed, i),
 as Sampler.sample(model, seed, i) draws it, on the device for all rows of a
-step at once. Greedy requests beside it keep their results.
+step at once. Greedy requests beside it keep their results. A request whose
+row has nothing to draw (every logit masked or NaN) ends there, with the
+tokens it has and error(rid) saying so; the others go on.
 
 Each step() first admits waiting requests into free slots (first come,
 first served: the slot is cleared, the prompt prefilled, its first token
@@ -40,6 +42,8 @@ import numpy as np
 
 from .model import Sampler, uniform
 
+NO_TOKEN = 0xFFFFFFFF  # what sample() gives for a row whose every logit is masked
+
 
 def _pool_empty(e: BaseException) -> bool:
     """The error a paged batch raises when its page pool has no page left."""
@@ -62,6 +66,7 @@ class _Request:
     seed: int = 0
     tokens: list = field(default_factory=list)
     done: bool = False
+    error: str | None = None  # why it ended early
     order: int = 0  # admission count when it took its slot
     restarts: int = 0  # times it was preempted
 
@@ -110,14 +115,24 @@ class Server:
         r = self.requests[rid]
         return list(r.tokens) if r.done else None
 
-    def _finish_if_done(self, slot: int) -> None:
+    def error(self, rid: int) -> str | None:
+        """Why the request ended before its tokens were all there, or None."""
+        return self.requests[rid].error
+
+    def _take(self, slot: int, token: int | None) -> None:
+        """The slot's next token (None: its row had nothing to draw)."""
         r = self.slots[slot]
-        if len(r.tokens) >= r.max_tokens or (r.eos is not None and r.tokens[-1] == r.eos):
-            r.done = True
-            self.slots[slot] = None
-            if self.paged:
-                self.kb.reset(slot)
-                self.used[slot] = False
+        if token is None:
+            r.error = "nothing to draw: every logit is masked"
+        else:
+            r.tokens.append(token)
+            if len(r.tokens) < r.max_tokens and (r.eos is None or token != r.eos):
+                return
+        r.done = True
+        self.slots[slot] = None
+        if self.paged:
+            self.kb.reset(slot)
+            self.used[slot] = False
 
     def _active(self) -> list[int]:
         return [i for i, r in enumerate(self.slots) if r is not None]
@@ -142,18 +157,18 @@ class Server:
                 if _pool_empty(e) and self._active():
                     return  # pages come back when an active request finishes
                 raise
-            r.tokens.append(first)
             r.order = self._admitted
             self._admitted += 1
             self.slots[slot] = r
-            self._finish_if_done(slot)
+            self._take(slot, first)
 
-    def _draw(self, requests) -> list[int]:
-        """The next token of every request, row i of the latest logits its."""
+    def _draw(self, requests) -> list[int | None]:
+        """The next token of every request, row i of the latest logits its;
+        None where every logit is masked."""
         greedy = Sampler.greedy()
         toks, _ = self.kb.sample([r.sampler or greedy for r in requests],
                                  [uniform(r.seed, len(r.tokens)) if r.sampler else 0.0 for r in requests])
-        return [int(t) for t in toks]
+        return [None if int(t) == NO_TOKEN else int(t) for t in toks]
 
     def _preempt(self, seqs: list[int]) -> None:
         """Return the pages of the most recently admitted of `seqs`; its
@@ -189,8 +204,7 @@ class Server:
             drawn = self._draw(rows)
             amax = [a if r.sampler is None else d for r, a, d in zip(rows, amax, drawn)]
         for i, t in zip(seqs, amax):
-            self.slots[i].tokens.append(int(t))
-            self._finish_if_done(i)
+            self._take(i, None if t is None else int(t))
         return len(seqs)
 
     def run(self) -> dict[int, list]:

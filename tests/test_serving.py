@@ -244,3 +244,52 @@ def test_sampled_requests_do_not_depend_on_their_neighbours():
     assert alone[0] == _alone(reqs[0][0], reqs[0][1])
     assert 0 <= min(uniform(s, o) for s in range(50) for o in range(50)) and max(
         uniform(s, o) for s in range(50) for o in range(50)) < 1
+
+
+class MaskedFake(SampledFake):
+    """Rows whose history ends in `bad` have every logit masked; a step refuses
+    tokens beyond the vocabulary, for all its rows."""
+
+    bad = 11
+
+    def decode_step_seqs(self, seqs, tokens, want_logits=True):
+        if any(not 0 <= int(t) < V for t in tokens):
+            raise RuntimeError(f"tensor index out of bounds: {tokens}")
+        return super().decode_step_seqs(seqs, tokens, want_logits)
+
+    def sample(self, samplers, u):
+        toks, logp = super().sample(samplers, u)
+        for i, s in enumerate(self.rows):
+            if self.hist[s][-1] == self.bad and samplers[i].temperature > 0:
+                toks[i], logp[i] = 0xFFFFFFFF, -np.inf
+        return toks, logp
+
+
+class PagedMaskedFake(MaskedFake):
+    def pages(self):
+        return (9, 9)
+
+
+@pytest.mark.parametrize("fake", [MaskedFake, PagedMaskedFake])
+def test_a_row_with_nothing_to_draw_ends_its_request_alone(fake):
+    from inferox_b200 import Sampler
+    sampler = Sampler(0.9, 5)
+    alone = {}
+    for i in range(60):  # what each request gives by itself
+        srv = Server(fake(1, 100))
+        rid = srv.submit([i + 20, 3], 25, sampler=sampler, seed=i)
+        alone[i] = (srv.run()[rid], srv.error(rid))
+    bad = [i for i in alone if alone[i][1]][:3]
+    good = [i for i in alone if not alone[i][1]][:5]
+    assert len(bad) == 3 and len(good) == 5 and all(len(alone[i][0]) == 25 for i in good)
+    assert all(alone[i][0][-1] == MaskedFake.bad and len(alone[i][0]) < 25 for i in bad)
+    srv = Server(fake(3, 100))
+    order = [bad[0], good[0], bad[1], good[1], good[2], bad[2], good[3], good[4]]
+    rids = [srv.submit([i + 20, 3], 25, sampler=sampler, seed=i) for i in order]
+    first = srv.submit([4, MaskedFake.bad], 9, sampler=sampler)  # masked at its prompt's last row
+    greedy = srv.submit([4, MaskedFake.bad], 9)
+    got = srv.run()
+    for i, rid in zip(order, rids):
+        assert (got[rid], srv.error(rid)) == alone[i] and srv.result(rid) == alone[i][0]
+    assert got[first] == [] and srv.error(first) and srv.result(first) == []
+    assert got[greedy] == _alone([4, MaskedFake.bad], 9) and srv.error(greedy) is None
