@@ -432,12 +432,12 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     const int pos = s.len - s.ql + (int)(prow - s.q0);
     const int jmax = prow >= 0 ? pos : INT32_MAX, jmin = prow >= 0 && a.window ? max(0, pos - a.window + 1) : 0;
     const int see_lo = __reduce_max_sync(0xffffffffu, jmin), see_hi = __reduce_min_sync(0xffffffffu, jmax);
-    float m = -INFINITY, l = 0.f, alpha = 0.f, weigh = 1.f;
+    float m = -INFINITY, l = 0.f, alpha = 0.f;
     float o[HALF];
 #pragma unroll
     for (int i = 0; i < HALF; ++i) o[i] = 0.f;
-    int kref = 1000;  // o counts in 2^-(1 + kref) (p times 2^10, nibbles in 2^-9): the smallest page exponent so far
-    auto add_output = [&](int turn) {  // o = o alpha + the page's sums, which count in the page's own exponent
+    int kref = 1000;  // o counts in 2^-(1 + kref) (p times 2^10, nibbles in 2^-9): the exponent of the last page with values
+    auto add_output = [&](int turn) {  // o = o alpha + the page's sums
       mbar_wait(&o_bar, o_phase, nullptr, 0);
       o_phase ^= 1;
       tc_after();
@@ -448,10 +448,6 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
         uint32_t r[16];
         tc_ld16(at + i, r);
         tc_wait_ld(r);
-        if (weigh != 1.f) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * weigh);
-        }
 #pragma unroll
         for (int k = 0; k < 16; ++k) o[i + k] = fmaf(o[i + k], alpha, __uint_as_float(r[k]));
       }
@@ -520,14 +516,12 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
         const float base = m2 == -INFINITY ? 0.f : m2;
         const float shrink = ex2(m - base);
         m = m2;
-        // what the page's sums count in is settled as they are added, in f32: a
-        // page of smaller values keeps every bit of its probabilities
-        float scale_o = shrink, scale_r = 1.f;
-        if (kval < kref) {
-          scale_o *= kref == 1000 ? 0.f : __uint_as_float((uint32_t)(127 + kval - kref) << 23);
+        // o goes over to what this page's sums count in, in f32 and by powers of
+        // two, so that no page costs another's bits (|o| stays below 2^90)
+        float scale_o = shrink;
+        if (kval != 1000) {
+          if (kref != 1000) scale_o *= __uint_as_float((uint32_t)(127 + kval - kref) << 23);
           kref = kval;
-        } else if (kval > kref && kval != 1000) {  // (of a page of zeros nothing is added)
-          scale_r = __uint_as_float((uint32_t)(127 + kref - kval) << 23);
         }
         // p enters times 2^10 = exp2(x f - (base - 10)); its sum is divided by that again
         const float down = base - 10.f;
@@ -545,7 +539,6 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
         l = fmaf(l, shrink, (sum[0] + sum[1]) * 0x1p-10f);
         if (j > j0) add_output(1);
         alpha = scale_o;
-        weigh = scale_r;
         tc_st16(mine + L::kPh + 16 * half, ph);
         tc_st16(mine + L::kPl + 16 * half, pl);
         unpack_values<NB>(sm, raw, rows_here, kval);
