@@ -433,12 +433,18 @@ ifx_status ifx_op_kv4_load(int type, const void *pages, size_t n_pages,
  * q_start[b + 1] - 1 (q_start [n_seqs + 1], rising from 0), or row b when
  * q_start is NULL (rows = n_seqs, one row per sequence). The last query row
  * sees all kv_len rows, the one before it one less, and so on; with
- * window > 0 each sees its last `window` rows only. softmax(scale q k) v in
- * f32 throughout; a row that sees nothing (kv_len 0, or a query row before
- * the cache's first) gives 0; rows of out that are no sequence's (before
- * q_start[0], behind q_start[n_seqs]) are left as they were, or set to 0 with
- * zero_rest. A table entry outside the pages hides its rows. At most
- * IFX_KV4_ATTENTION_MAX_SEQS sequences.
+ * window > 0 each sees its last `window` rows only. A row that sees nothing
+ * (kv_len 0, or a query row before the cache's first) gives 0; rows of out
+ * that are no sequence's (before q_start[0], behind q_start[n_seqs]) are left
+ * as they were, or set to 0 with zero_rest. A table entry outside the pages
+ * hides its rows. At most IFX_KV4_ATTENTION_MAX_SEQS sequences.
+ * softmax(scale q k) v: scores, maxima, sums and outputs are f32. With few
+ * query rows per kv head a query enters the products with 22 bits below its
+ * head's largest value, and a probability times a value's scale to 2^-20 of
+ * the largest such term of a page in the same block of 32 dimensions; with
+ * many, queries and probabilities have 22 bits each, and a block whose values
+ * are below 2^-19 of the page's largest loses bits. Equal calls repeat bit for
+ * bit; a row's last bits may change with the other rows of its call.
  * ws: scratch of at least ifx_kv4_attention_workspace bytes, 256-byte
  * aligned, any contents, for one call at a time. */
 size_t ifx_kv4_attention_workspace(size_t n_heads, size_t n_kv_heads,

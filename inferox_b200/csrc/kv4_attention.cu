@@ -18,7 +18,11 @@
 // Precision. The other operand enters as fixed point of 23 bits in three
 // byte planes: a query head scaled so that its largest magnitude is 4.1e6,
 // and p dV, with p relative to its page's own maximum, scaled
-// so that 1 * the page's largest dV is 4.1e6. Products
+// so that 1 * the page's largest dV is 4.1e6. Where a page's dV differ by more
+// than a factor of 8 that would cost the small ones their bits, to a row that
+// is hidden, weighs nothing or is large in other dimensions: there every
+// query's own largest p dV of a block takes the range, by a power of two (a
+// page costs 20% more). A step is at most 2^-19 of that largest term. Products
 // and their sums over a block (keys) or a page (values) are exact integers;
 // block scales, scores, maxima, sums and outputs are f32.
 //
@@ -85,6 +89,8 @@ constexpr uint32_t kHigh = 0xf0f0f0f0u, kSign = 0x80808080u;
 // signed top digit.
 constexpr float kMagic = 12582912.f;
 constexpr float kTop = 4.1e6f;
+constexpr float kUneven = 8.f;  // ratio of a page's value scales from which on every block has a range of its own
+constexpr int kMaxLift = 60;    // (f16 scales are at most 2^40 apart; p dV 2^60 stays far below f32's end)
 
 // 65536 top + 256 mid + low of the three planes' sums; top comes doubled.
 __device__ __forceinline__ float planes(int top2, int mid, int low) {
@@ -360,19 +366,21 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
           fpage = page_at();
         }
         // rows that hold nothing (behind the last one, or of a page that does
-        // not exist) get scale 0, whatever bytes are there
+        // not exist) get scale 0, whatever bytes are there; as values that of the
+        // page's first row, since a small one would make the page uneven
         const int live_rows = here ? len - row0 : 0;
         const bool clear = live_rows < kKv4PageRows;
-        auto wipe = [&](uint8_t *buf) {
+        auto wipe = [&](uint8_t *buf, bool first) {
           for (int r = max(0, live_rows) + lane; r < kKv4PageRows; r += 32)
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-              reinterpret_cast<uint16_t *>(buf + r / kKv4TileRows * HB + SC)[r % kKv4TileRows * NB + b] = 0;
+              reinterpret_cast<uint16_t *>(buf + r / kKv4TileRows * HB + SC)[r % kKv4TileRows * NB + b] =
+                  first && live_rows > 0 ? reinterpret_cast<const uint16_t *>(buf + SC)[b] : 0;
           __syncwarp();
         };
         // ---- scores
         mbar_wait(&bar[0], phase, nullptr, 0);
-        if (clear) wipe(kbuf);
+        if (clear) wipe(kbuf, false);
         float sc[4][NT][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -423,19 +431,22 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
         // ---- the page's maxima of value scales and scores, the running maximum
         mbar_wait(&bar[1], phase, nullptr, 0);
         phase ^= 1;
-        if (clear) wipe(vbuf);
-        uint32_t top = 0;
+        if (clear) wipe(vbuf, true);
+        uint32_t top = 0, low = 0x7fff7fffu;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < 8 * NB; e += 32)
             if (8 * NB % 32 == 0 || e + lane < 8 * NB) {
-              const uint32_t w = reinterpret_cast<const uint32_t *>(vbuf + i * HB + SC)[e + lane];
-              top = __vmaxu2(top, w & 0x7fff7fffu);
+              const uint32_t w = reinterpret_cast<const uint32_t *>(vbuf + i * HB + SC)[e + lane] & 0x7fff7fffu;
+              top = __vmaxu2(top, w);
+              low = __vminu2(low, w);
             }
         top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+        low = __reduce_min_sync(0xffffffffu, min(low & 0xffffu, low >> 16));
         const float dmax = __half2float(__ushort_as_half((uint16_t)min(top, 0x7bffu)));
         const float ps = top ? kTop / dmax : 0.f;
+        const bool uneven = kUneven * __half2float(__ushort_as_half((uint16_t)min(low, 0x7bffu))) < dmax;
         float beta[NT], share[NT], base[NT];  // of this page's p dV and p in the running sums
         bool moved = false;
 #pragma unroll
@@ -465,9 +476,32 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
               for (int i = 0; i < 4; ++i) o[nt][b][i] *= beta[nt];
         }
         // ---- probabilities
+        uint32_t lifts = 0;  // a byte per column tile: sc counts in 2^lift times ps, beta in its reciprocal
+        auto power = [](int e) { return __uint_as_float((uint32_t)(127 + e) << 23); };
+        // how far a block's largest term of every query lies below the range
+        auto room = [&](int b, int (&by)[NT], auto term) {
+          float most[NT] = {};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint16_t *eb = reinterpret_cast<const uint16_t *>(vbuf + i * HB + SC) + g * NB + b;
+            const float ea = fabsf(h2f(eb[0])), ec = fabsf(h2f(eb[8 * NB]));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) most[nt] = fmaxf(most[nt], fmaxf(term(i, nt, 0) * ea, term(i, nt, 1) * ec));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float x = quad_rows_max(most[nt]);
+            const int was = (int)(lifts >> (8 * nt) & 255u);
+            by[nt] = x > 0.f ? max(0, min(kMaxLift, was + (int)(__float_as_uint(__fdividef(kTop, x)) >> 23) - 127)) - was : 0;
+            lifts += (uint32_t)by[nt] << (8 * nt);
+          }
+        };
+        int first[NT] = {};
+        if (uneven) room(0, first, [&](int i, int nt, int r) { return ex2(sc[i][nt][r] - base[nt]) * ps; });
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          beta[nt] = share[nt] * dmax * (1.f / (16.f * kTop));
+          beta[nt] = share[nt] * dmax * (1.f / (16.f * kTop)) * power(-first[nt]);
+          const float pl = ps * power(first[nt]);
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -475,7 +509,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
             for (int r = 0; r < 2; ++r) {
               const float p = ex2(sc[i][nt][r] - base[nt]);
               sum += p;
-              sc[i][nt][r] = p * ps;
+              sc[i][nt][r] = p * pl;
             }
           l[nt] = fmaf(share[nt], sum, l[nt]);
         }
@@ -488,6 +522,19 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+          if (b > 0 && uneven) {
+            int by[NT];
+            room(b, by, [&](int i, int nt, int r) { return sc[i][nt][r]; });
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              beta[nt] *= power(-by[nt]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                sc[i][nt][0] *= power(by[nt]);
+                sc[i][nt][1] *= power(by[nt]);
+              }
+            }
+          }
           uint32_t lo[NT][4], hi[TT][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {

@@ -25,15 +25,15 @@ def own_bound(q, K, V, lens, start, scale, window=0):
     """The result in 64 bits, and a bound from what each row sees itself: a
     score's error as in test_gpu_serve_ops.bound, and twice that of a
     probability; 2^-20 for the exponential and the planes of 22 bits; per
-    page of 64 rows fixed-point steps of 2^-21 (half of 4 / 4.1e6) of the
-    largest term, eight deviations of 64 of them, which f32's own sums stay
-    below; relative to the magnitudes summed, at their largest in a block of
-    32 dimensions (its largest value is what a block's scale is made for)."""
+    page of 64 rows fixed-point roundings of 2^-20 (half of 8 / 4.1e6) of the
+    largest term, eight deviations of 64 of them; f32's sums; relative to the
+    magnitudes summed, at their largest in a block of 32 dimensions (its
+    largest value is what a block's scale is made for)."""
     ref, worst = SR.attention(q, K, V, lens, start, scale, window)
     mag = SR.attention(q, K, [np.abs(v) for v in V], lens, start, scale, window)[0]
     mag = np.repeat(mag.reshape(*mag.shape[:-1], -1, 32).max(-1), 32, -1)
     n, hd = max(lens), q.shape[-1]
-    rel = 2 * (hd + 16) * 2.0 ** -24 * worst + 2.0 ** -20 + 8 * 8 * 2.0 ** -21 / 3 ** 0.5 + 8 * np.sqrt(n + 1) * 2.0 ** -24
+    rel = 2 * (hd + 16) * 2.0 ** -24 * worst + 2.0 ** -20 + 8 * 8 * 2.0 ** -20 / 3 ** 0.5 + 8 * np.sqrt(n + 1) * 2.0 ** -24
     return ref, mag * rel + np.abs(ref) * 2.0 ** -24
 
 
@@ -96,3 +96,35 @@ def test_attention_pages_of_unequal_values(H, G, hd, ql, big_first, low):
     q, start = ones_first(rng, seqs * ql, H, hd), ql * np.arange(seqs + 1)
     ref, lim = own_bound(q, K, V, [n] * seqs, start, 1.0)
     close(ops.kv4_attention(cuda(q), pages, i32(table), i32([n] * seqs), G, q_start=i32(start), scale=1.0), ref, lim)
+
+
+@pytest.mark.parametrize("H,G,hd", [(4, 2, 64), (8, 1, 128), (4, 1, 96), (2, 2, 256)])
+@pytest.mark.parametrize("ql", [1, 5, 128])
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_blocks_and_rows_of_unequal_values(H, G, hd, ql, window):
+    """Blocks of 32 dimensions 1e4 apart in size, held dimension by dimension,
+    and rows 1e4 times larger than the others: outside the window, behind the
+    query row, or with hardly any weight. None of them costs the rest."""
+    rng = np.random.default_rng(hd + ql + window)
+    lens = [150, 64, 39, 260]
+    pages, table, K, V = filled(rng, lens, G, hd)
+    start = ql * np.arange(len(lens) + 1)
+    q = ones_first(rng, start[-1], H, hd)
+    for kind in range(4):
+        for b, n in enumerate(lens):
+            s, v = rng.uniform(-2, 0, n), rng.standard_normal((n, G, hd))
+            if kind == 0:
+                v *= np.repeat(10.0 ** rng.uniform(-4, 0, (1, G, hd // 32)), 32, -1)
+            elif kind == 1:  # a block each, of rows that hardly weigh
+                for j in rng.integers(0, n, 5):
+                    s[j] = -40
+                    v[j, :, :32 * rng.integers(1, hd // 32 + 1)] *= 1e4
+            elif kind == 2:  # hidden from every row, or from all but the last
+                v[: max(0, n - ql - window + 1) if window else 0] *= 1e4
+                v[n - ql + 1:] *= 1e4 if ql > 1 else 1
+            else:
+                v *= 10.0 ** rng.uniform(-4, 0, (n, 1, 1))
+            K[b], V[b] = store(pages, table, b, spread(rng, n, G, hd, s), v)
+        ref, lim = own_bound(q, K, V, lens, start, 1.0, window)
+        got = ops.kv4_attention(cuda(q), pages, i32(table), i32(lens), G, q_start=i32(start), scale=1.0, window=window)
+        close(got, ref, lim)
