@@ -361,7 +361,9 @@ ifx_status ifx_op_sample_u_static(const float *logits_dev, size_t n,
  * cache pages: pages and row slots for the rows that arrive, the rows into
  * the cache, attention over it, the next tokens. All pointers are device
  * memory of the current device; every call only enqueues work on `stream`
- * and may be captured into a graph. Counts and indices are int32.
+ * and may be captured into a graph. Counts and indices are int32. Waits
+ * inside a kernel are bounded; should one give up, the rows that it held up
+ * come out as NaN, a sampled token as -1 with logprob NaN.
  *
  * A page has IFX_PAGE_ROWS rows. Row `pos` of a sequence lies in the page
  * table[seq * max_pages + pos / 64]; its slot is page * 64 + pos % 64. */

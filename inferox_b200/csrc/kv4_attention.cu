@@ -252,6 +252,9 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
 
     int left = (int)(u1 - u0);
     uint32_t phase = 0;
+    // a copy did not come: seen by this lane, and (from the next vote on) by the
+    // warp; then nothing more is asked for, and what is open gets NaN
+    bool came = true, lost = false;
     const int czero[4] = {0, 0, 0, 0};
     while (left > 0) {
       // ---- query columns of this segment: lane (g, t) holds column g, that
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
       int row0 = (s.lo + (int)(at - s.begin)) * kKv4PageRows;
       int todo = min(left, (int)(s.end - at));
       left -= todo;
-      for (; todo > 0; --todo, row0 += kKv4PageRows) {
+      for (; todo > 0 && !lost; --todo, row0 += kKv4PageRows) {
         // the cursor moves to the next page (its table entry is on its way
         // while this page's keys are multiplied)
         const bool here = ok;
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
           __syncwarp();
         };
         // ---- scores
-        mbar_wait(&bar[0], phase, nullptr, 0);
+        came = mbar_wait(&bar[0], phase, nullptr, 0);
         if (clear) wipe(kbuf, false);
         float sc[4][NT][2];
 #pragma unroll
@@ -415,7 +418,12 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
           }
         }
         if (clear) fence_proxy_async_smem();  // the scales written above, before the next copy
-        __syncwarp();
+        lost = !__all_sync(0xffffffffu, came);
+        if (lost) {  // (copies on their way write this CTA's memory)
+          mbar_wait(&bar[0], phase, nullptr, 0);
+          mbar_wait(&bar[1], phase, nullptr, 0);
+          break;
+        }
         copy(0, more);
         if (!here || row0 < see_lo || row0 + kKv4PageRows - 1 > see_hi) {
 #pragma unroll
@@ -429,7 +437,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
           }
         }
         // ---- the page's maxima of value scales and scores, the running maximum
-        mbar_wait(&bar[1], phase, nullptr, 0);
+        came = mbar_wait(&bar[1], phase, nullptr, 0);
         phase ^= 1;
         if (clear) wipe(vbuf, true);
         uint32_t top = 0, low = 0x7fff7fffu;
@@ -584,7 +592,12 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
           }
         }
         if (clear) fence_proxy_async_smem();
-        __syncwarp();
+        lost = !__all_sync(0xffffffffu, came);
+        if (lost) {
+          mbar_wait(&bar[1], phase ^ 1, nullptr, 0);
+          if (more) mbar_wait(&bar[0], phase, nullptr, 0);
+          break;
+        }
         copy(1, more);
         ok = (unsigned)fpage < (unsigned)a.n_pages;
       }
@@ -596,7 +609,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
       float *part = L::part(sm, slot);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float sum = quad_rows_sum(l[nt]);
+        const float sum = lost ? __uint_as_float(0x7fc00000u) : quad_rows_sum(l[nt]);
         int head;
         const long long row = pair_row<PAIRS>(a, s.q0, s.ql, s.ct, 4 * nt + t, &head);
         const float f = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
@@ -627,6 +640,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) kv4_attn_kernel(const __grid_co
         __syncwarp();
       }
     }
+    if (lost && lane == 0 && a.err) atomicExch(a.err, kErrKv4);
   }
   __syncthreads();
 

@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
   constexpr int HD = L::HD, ROWS = kTcRows, HALF = 16 * NB;
   extern __shared__ __align__(128) uint8_t sm[];
   long long *pre = reinterpret_cast<long long *>(sm + L::kBytes);
-  __shared__ __align__(8) uint64_t raw_bar[2], s_bar, o_bar;
+  __shared__ __align__(8) uint64_t raw_bar[2], s_bar, o_bar, end_bar[2];
+  __shared__ int s_sent;  // copies asked for
   __shared__ uint32_t tmem_slot;
   __shared__ long long s_scan[kTcThreads / 32], s_tiles[kTcThreads / 32];
   __shared__ float s_both[2][ROWS], s_sum[2][ROWS];  // what the two threads of a row exchange: largest values, sums
@@ -247,6 +248,9 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     mbar_init(&raw_bar[1], 1);
     mbar_init(&s_bar, 1);
     mbar_init(&o_bar, 1);
+    mbar_init(&end_bar[0], 1);
+    mbar_init(&end_bar[1], 1);
+    s_sent = 0;
     fence_mbar_init();
   }
   pdl_launch();
@@ -329,6 +333,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     } else {
       mbar_arrive(&raw_bar[st]);
     }
+    ++s_sent;
     ++fu;
     look();
   };
@@ -366,11 +371,15 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
   int st = 0;
   uint32_t phase = 0, s_phase = 0, o_phase = 0;
   long long u = u0;
+  // a wait gave up: in this thread, which waits for nothing more then (and
+  // thread 64 asks for nothing), and, from a segment's end on, in any of the
+  // CTA: that segment and the ones behind it get NaN
+  bool ok = true, lost = false;
   while (u < u1) {
     int head;
     const long long prow = pair_row<ROWS>(a, s.q0, s.ql, s.ct, row, &head);
-    float qs;
-    {
+    float qs = 0.f;
+    if (!lost) {
       // ---- half of the thread's query row, two f16 planes, scaled by a power
       // of two that puts the row's largest magnitude into [2^10, 2^11)
       float x[HALF];
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     for (int i = 0; i < HALF; ++i) o[i] = 0.f;
     int kref = 1000;  // o counts in 2^-(1 + kref) (p times 2^10, nibbles in 2^-9): the exponent of the last page with values
     auto add_output = [&](int turn) {  // o = o alpha + the page's sums
-      mbar_wait(&o_bar, o_phase, nullptr, 0);
+      ok = ok && mbar_wait(&o_bar, o_phase, nullptr, 0);
       o_phase ^= 1;
       tc_after();
       if (L::kTwice && half != turn) return;
@@ -460,11 +469,11 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     seen_units(a, s, &first, &stop);
     first = max(first, u);
     stop = min(stop, u1);
-    if (first < stop) {
+    if (first < stop && !lost) {
       int j = s.lo + (int)(first - s.begin);
       const int j0 = j, j1 = j + (int)(stop - first);
       int rows_here = rows_of(page_at(j), j), coming = j + 1 < j1 ? page_at(j + 1) : -1;
-      mbar_wait(&raw_bar[st], phase, nullptr, 0);
+      ok = ok && mbar_wait(&raw_bar[st], phase, nullptr, 0);
       int2 ks = page_exponents<NB>(sm + st * L::kRaw, rows_here);
       unpack_keys<NB>(sm, sm + st * L::kRaw, rows_here, ks.x);
       fence_async();
@@ -475,7 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
         const uint8_t *raw = sm + st * L::kRaw;
         const bool next = j + 1 < j1;
         const int row0 = j * kKv4PageRows + 32 * half;  // this thread's 32 keys
-        mbar_wait(&s_bar, s_phase, nullptr, 0);
+        ok = ok && mbar_wait(&s_bar, s_phase, nullptr, 0);
         s_phase ^= 1;
         tc_after();
         uint32_t sr[32];
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
         if (next) {
           rows_next = rows_of(coming, j + 1);
           if (j + 2 < j1) coming = page_at(j + 2);
-          mbar_wait(&raw_bar[st ^ 1], phase ^ (uint32_t)st, nullptr, 0);
+          ok = ok && mbar_wait(&raw_bar[st ^ 1], phase ^ (uint32_t)st, nullptr, 0);
           ks_next = page_exponents<NB>(sm + (st ^ 1) * L::kRaw, rows_next);
           unpack_keys<NB>(sm, sm + (st ^ 1) * L::kRaw, rows_next, ks_next.x);
         }
@@ -547,7 +556,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
         tc_before();
         __syncthreads();  // probabilities and values are in place, the page is read
         if (tid == ROWS) issue_output(0);
-        if (tid == 64) fetch(st);
+        if (tid == 64 && ok) fetch(st);
         rows_here = rows_next;
         ks = ks_next;
         phase ^= (uint32_t)st;
@@ -563,8 +572,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
     }
     // ---- the segment's end, or the range's: the result, or a partial
     s_sum[half][row] = l;
-    __syncthreads();
-    const float sum = s_sum[0][row] + s_sum[1][row];
+    lost = __syncthreads_or(!ok);
+    const float sum = lost ? __uint_as_float(0x7fc00000u) : s_sum[0][row] + s_sum[1][row];
     const bool whole = s.begin >= u0 && s.end <= u1;
     const float unit = kref == 1000 ? 0.f : __uint_as_float((uint32_t)max(0, 127 - 1 - kref) << 23);
     const float f = !whole ? unit : sum == 0.f ? 0.f : unit / sum;
@@ -591,6 +600,15 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<NB>::kPerSm) kv4_attn_tc_k
       __syncthreads();  // the sums are read
       s = locate<ROWS>(a, pre, u);
     }
+  }
+  if (lost) {  // products and copies on their way use this CTA's memories
+    if (tid == 0 && a.err) atomicExch(a.err, kErrKv4Chunk);
+    if (tid == 0 || tid == ROWS) {  // (the two threads that issue products)
+      tc_commit(&end_bar[tid / ROWS]);
+      mbar_wait(&end_bar[tid / ROWS], 0, nullptr, 0);
+    }
+    if (tid == 64)
+      for (int i = max(0, s_sent - 2); i < s_sent; ++i) mbar_wait(&raw_bar[i & 1], (uint32_t)(i >> 1) & 1u, nullptr, 0);
   }
   tc_before();
   __syncthreads();

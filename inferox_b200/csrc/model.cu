@@ -1304,6 +1304,7 @@ ifx_status Model::enqueue_decode_batch(KvBatch &kb, cudaStream_t st, int n, cons
       a.hd = hd;
       a.scale = 1.0f / sqrtf((float)hd);
       a.ws = kb.ws4;
+      a.err = err;
       IFX_TRY(op_kv4_attention(a, st));
     } else {
       DecodeAttnArgs a{};
@@ -1498,12 +1499,13 @@ ifx_status Model::sample_batch(KvBatch *kb, int n, const ifx_sampler *s, const f
   float *b = sample_buf, *o = b + (size_t)5 * rows;
   const int64_t V = (int64_t)cfg.vocab_size;
   SampleRowsArgs a{kb ? kb->logits : logits, rows, V, V, b, b + rows, reinterpret_cast<int *>(b + 2 * rows),
-                   b + 3 * rows, b + 4 * rows, reinterpret_cast<int *>(o), o + rows};
+                   b + 3 * rows, b + 4 * rows, reinterpret_cast<int *>(o), o + rows, err};
   IFX_TRY(op_sample_rows(a, st));
   IFX_CUDA(cudaMemcpyAsync(out.data(), o, out.size() * sizeof(float), cudaMemcpyDeviceToHost, st));
   IFX_TRY(step_sync(st));
   for (int i = 0; i < n; ++i) {
     const int r = kb ? kb->order[(size_t)i] : 0;
+    if (std::isnan(out[(size_t)(rows + r)])) IFX_TRY(check_err());  // (a row always has a logprob)
     memcpy(&tokens[i], &out[(size_t)r], sizeof(uint32_t));
     if (logprobs) logprobs[i] = out[(size_t)(rows + r)];
   }

@@ -52,6 +52,8 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
+constexpr uint32_t kLost = 0xffffffffu;  // in place of a largest value's bits (a NaN's, which no maximum has)
+
 __device__ const double kPow2[32] = {  // 2^(j / 32)
     1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
     1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   if (IN_SMEM && wide) {
     // kept as it is: a NaN is in no bucket and has no weight, -0 equals +0
     // until the sort
-    mbar_wait(&bar, 0, nullptr, 0);
+    if (!mbar_wait(&bar, 0, a.err, kErrSample)) atomicMax(&sh.best, (u64)kLost);
 #pragma unroll 4
     for (int i = tid; i < len / 4; i += kThreads) {
       const float4 v = reinterpret_cast<const float4 *>(zs)[i];
@@ -673,7 +675,19 @@ __global__ void __launch_bounds__(kThreads, PER_SM) sample_rows_kernel(const __g
   const float scale = (float)(kBuckets - 1) / (float)r.cut;
   const double u = fmin(fmax((double)u_row, 0.0), 1.0);
   cluster.sync();
-  r.zmax = unordered(__reduce_max_sync(0xffffffffu, lane < C ? (uint32_t)cluster.map_shared_rank(&sh, lane)->best : 0u));
+  const uint32_t most = __reduce_max_sync(0xffffffffu, lane < C ? (uint32_t)cluster.map_shared_rank(&sh, lane)->best : 0u);
+  if (most == kLost) {
+    // a copy did not come: no token, and no CTA leaves before its copy is over
+    // and the others have read that
+    if (IN_SMEM && wide) mbar_wait(&bar, 0, nullptr, 0);
+    if (rank == 0 && tid == 0) {
+      a.token[row] = -1;
+      if (a.logprob) a.logprob[row] = __uint_as_float(0x7fc00000u);
+    }
+    cluster.sync();
+    return;
+  }
+  r.zmax = unordered(most);
   // (no infinity counts but as the maximum)
   r.zcut = r.zmax == INFINITY ? INFINITY : fmaxf((float)((double)r.zmax - 1.01 * r.cut), -3.402823466e38f);
   const bool none = r.zmax == -INFINITY;

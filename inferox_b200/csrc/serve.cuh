@@ -39,6 +39,10 @@ struct Kv4Layout {
 inline bool kv4_head_dim_ok(size_t hd) { return hd >= 32 && hd <= 256 && hd % 32 == 0; }
 inline size_t kv4_page_bytes(size_t G, size_t hd) { return G * (size_t)Kv4Layout::head_bytes((int)(hd / 32)); }
 
+// A wait of these kernels that gives up sets `err` where there is one; the rows
+// that it held up come out as NaN (tokens as -1 with a NaN beside them).
+constexpr int kErrKv4 = 601, kErrKv4Chunk = 602, kErrSample = 603;
+
 // Raises a kernel's shared-memory limit, once per device: `done` holds a bit
 // for each (the call costs a microsecond or two).
 template <typename K>
@@ -103,6 +107,7 @@ struct Kv4AttnArgs {
   void *ws;
   bool zero_rest = false;     // rows of out that are no sequence's become 0
   bool alone = false;         // set by the launch: a CTA per segment
+  int *err = nullptr;         // device word that a wait which gives up sets
 };
 ifx_status op_kv4_attention(const Kv4AttnArgs &a, cudaStream_t st);
 // Bytes of scratch a call with these shapes needs.
@@ -116,6 +121,7 @@ struct SampleRowsArgs {
   const float *top_p, *min_p;
   int *token;
   float *logprob;
+  int *err = nullptr;
 };
 ifx_status op_sample_rows(const SampleRowsArgs &a, cudaStream_t st);
 
