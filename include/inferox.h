@@ -379,8 +379,9 @@ ifx_status ifx_op_sample_u_static(const float *logits_dev, size_t n,
  * new row slots, positions and seqs [max_tokens] (the last two nullable),
  * -1 behind the last row. status [1]: 0, or why nothing was taken and every
  * slot is -1, lens_out = lens, n_free_out = n_free and q_start 0:
- * 1 too few free pages, 2 a sequence longer than max_pages pages, 3 more
- * than max_tokens rows. Inputs and outputs do not overlap (lens_out may not
+ * 1 too few free pages, 2 a sequence longer than max_pages pages (with its new
+ * rows or without), 3 more than max_tokens rows. Lengths and counts below 0
+ * are 0. Inputs and outputs do not overlap (lens_out may not
  * be lens, nor n_free_out n_free: swap them from step to step); free_pages
  * [n_pages] is not written. At most IFX_PAGES_MAX_SEQS sequences. */
 ifx_status ifx_op_pages_extend(const int32_t *lens, const int32_t *add,

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const __gri
   int bad = 0;
   for (int b = b0; b < b1; ++b) {
     const int len = (int)min((long long)max(a.lens[b], 0), cap), add = max(a.add[b], 0);
-    if ((long long)len + add > cap) bad = 2;
+    if ((long long)max(a.lens[b], 0) + add > cap) bad = 2;
     ln[b] = len;
     qs[b] = add;
     tok += add;

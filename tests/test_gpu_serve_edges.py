@@ -128,3 +128,21 @@ def test_attention_blocks_and_rows_of_unequal_values(H, G, hd, ql, window):
         ref, lim = own_bound(q, K, V, lens, start, 1.0, window)
         got = ops.kv4_attention(cuda(q), pages, i32(table), i32(lens), G, q_start=i32(start), scale=1.0, window=window)
         close(got, ref, lim)
+
+
+# ----------------------------------------------------------------- pages
+@pytest.mark.parametrize("lens,add", [([300, 5], [0, 1]), ([257], [0]), ([2 ** 31 - 1, 0], [0, 0]), ([2 ** 31 - 1], [2 ** 31 - 1])])
+def test_extend_refuses_lengths_beyond_the_table(lens, add):
+    """A length that the table's row cannot hold is status 2 without new rows too."""
+    table = i32(np.arange(4 * len(lens)).reshape(-1, 4))
+    r = ops.pages_extend(i32(lens), i32(add), table, i32([90, 91, 92]), i32([3]), 8)
+    assert int(r.status) == 2 and r.lens.tolist() == lens and int(r.n_free) == 3
+    assert (r.slots == -1).all() and not r.q_start.any() and torch.equal(table, i32(np.arange(4 * len(lens)).reshape(-1, 4)))
+    r = ops.pages_extend(i32([256]), i32([0]), table[:1], i32([90]), i32([1]), 8)
+    assert int(r.status) == 0 and r.lens.tolist() == [256]
+
+
+def test_extend_counts_below_zero_are_zero():
+    r = ops.pages_extend(i32([-5, 70]), i32([2, -3]), i32([[-1, -1], [1, 0]]), i32([7, 8]), i32([2]), 4)
+    assert int(r.status) == 0 and r.lens.tolist() == [2, 70] and int(r.n_free) == 1
+    assert r.slots.tolist() == [8 * 64, 8 * 64 + 1, -1, -1] and r.q_start.tolist() == [0, 2, 2]
