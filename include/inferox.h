@@ -381,7 +381,7 @@ ifx_status ifx_op_sample_u_static(const float *logits_dev, size_t n,
  * slot is -1, lens_out = lens, n_free_out = n_free and q_start 0:
  * 1 too few free pages, 2 a sequence longer than max_pages pages (with its new
  * rows or without), 3 more than max_tokens rows. Lengths and counts below 0
- * are 0. Inputs and outputs do not overlap (lens_out may not
+ * are 0; a page number that no 32-bit slot can name gives slot -1. Inputs and outputs do not overlap (lens_out may not
  * be lens, nor n_free_out n_free: swap them from step to step); free_pages
  * [n_pages] is not written. At most IFX_PAGES_MAX_SEQS sequences. */
 ifx_status ifx_op_pages_extend(const int32_t *lens, const int32_t *add,

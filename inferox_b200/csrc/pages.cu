@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const __gri
       pos = ln[b] + ((int)i - qs[b]);
       const int held = pages_of(ln[b]), j = pos / kKv4PageRows;
       const int page = j < held ? a.table[(size_t)b * a.max_pages + j] : a.free_pages[n_free - 1 - (ps[b] + j - held)];
-      slot = page >= 0 ? page * kKv4PageRows + pos % kKv4PageRows : -1;
+      slot = (unsigned)page <= INT32_MAX / kKv4PageRows ? page * kKv4PageRows + pos % kKv4PageRows : -1;
     }
     a.slots[i] = slot;
     if (a.positions) a.positions[i] = pos;

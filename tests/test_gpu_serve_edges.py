@@ -146,3 +146,14 @@ def test_extend_counts_below_zero_are_zero():
     r = ops.pages_extend(i32([-5, 70]), i32([2, -3]), i32([[-1, -1], [1, 0]]), i32([7, 8]), i32([2]), 4)
     assert int(r.status) == 0 and r.lens.tolist() == [2, 70] and int(r.n_free) == 1
     assert r.slots.tolist() == [8 * 64, 8 * 64 + 1, -1, -1] and r.q_start.tolist() == [0, 2, 2]
+
+
+@pytest.mark.parametrize("page", [1 << 25, 1 << 26, (1 << 26) + 1, 2 ** 31 - 1, -1, -(2 ** 31)])
+def test_extend_of_impossible_pages_names_no_slot(page):
+    """page * 64 would pass 32 bits and name another page's rows."""
+    add = i32([3, 2])
+    r = ops.pages_extend(i32([5, 64]), add, i32([[page, -1], [0, -1]]), i32([4, page]), i32([2]), 6)
+    assert int(r.status) == 0 and r.slots.tolist() == [-1] * 6
+    r = ops.pages_extend(i32([5, 64]), add, i32([[(1 << 25) - 1, -1], [0, -1]]), i32([4, 3]), i32([2]), 6)
+    last = 64 * ((1 << 25) - 1)
+    assert r.slots.tolist() == [last + 5, last + 6, last + 7, 192, 193, -1]
