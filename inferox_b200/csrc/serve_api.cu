@@ -135,10 +135,12 @@ ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride, size_t
     IFX_CUDA(cudaMemset2DAsync(out, out_stride * ts, 0, w * ts, rows, S(stream)));
     return IFX_OK;
   }
+  // a window that no sequence outgrows is none (and differences with one stay within 32 bits)
+  const int seen = window >= max_pages * kKv4PageRows ? 0 : (int)window;
   Kv4AttnArgs a{q, out, type, (int64_t)q_stride, (int64_t)out_stride, (int64_t)rows,
                 static_cast<const uint8_t *>(pages), (int64_t)n_pages, table, kv_len, q_start, (int)max_pages,
                 (int)n_seqs, (int)n_heads, (int)n_kv_heads, (int)head_dim,
-                (int)(window > kIntMax ? 0 : window), scale, ws, zero_rest != 0 && q_start};
+                seen, scale, ws, zero_rest != 0 && q_start};
   return op_kv4_attention(a, S(stream));
 }
 

@@ -130,6 +130,23 @@ def test_attention_blocks_and_rows_of_unequal_values(H, G, hd, ql, window):
         close(got, ref, lim)
 
 
+@pytest.mark.parametrize("H,G,hd,ql", [(8, 4, 64, 128), (8, 4, 256, 128), (8, 1, 128, 9), (4, 2, 64, 1)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 60, 2 ** 40, 256, 255, 300])
+def test_attention_windows_longer_than_the_cache(H, G, hd, ql, window):
+    """As without one, also for more query rows than cached ones (256 and 300:
+    longer than any sequence of the table, or just so)."""
+    rng = np.random.default_rng(ql)
+    lens = [100, 200, 3, 0] * 4
+    pages, table, K, V = filled(rng, lens, G, hd)
+    start = ql * np.arange(len(lens) + 1)
+    q = cuda(rng.standard_normal((start[-1], H, hd)).astype(np.float32))
+    args = (q, pages, i32(table), i32(lens), G)
+    kw = dict(q_start=i32(start))
+    assert torch.equal(ops.kv4_attention(*args, **kw, window=window), ops.kv4_attention(*args, **kw))
+    ref, lim = own_bound(q.cpu().numpy(), K, V, lens, start, hd ** -0.5, min(window, 1000))
+    close(ops.kv4_attention(*args, **kw, window=window), ref, lim)
+
+
 # ----------------------------------------------------------------- pages
 @pytest.mark.parametrize("lens,add", [([300, 5], [0, 1]), ([257], [0]), ([2 ** 31 - 1, 0], [0, 0]), ([2 ** 31 - 1], [2 ** 31 - 1])])
 def test_extend_refuses_lengths_beyond_the_table(lens, add):
