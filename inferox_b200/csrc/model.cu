@@ -218,10 +218,14 @@ __global__ void kv_read_kernel(const __half *c, float *out, int len, int G, int 
   }
 }
 
+// Zeroed memory. The fill runs on the default stream, behind whatever the
+// caller's program has there, and the model's stream does not wait for that
+// one: it is waited for here.
 template <typename T>
 ifx_status dalloc(T **p, size_t n) {
   IFX_CUDA(cudaMalloc(reinterpret_cast<void **>(p), std::max<size_t>(n, 1) * sizeof(T)));
   IFX_CUDA(cudaMemset(*p, 0, std::max<size_t>(n, 1) * sizeof(T)));
+  IFX_CUDA(cudaStreamSynchronize(nullptr));
   return IFX_OK;
 }
 

@@ -81,3 +81,29 @@ def test_greedy_loop_leaves_its_last_rows():
             kb.prefill(s, synth.prompt_ids(2048, 20 + s, seed=s), True)
         out, _ = kb.decode_greedy([7, 8], 5)
         assert _greedy(kb, 2) == [int(t) for t in out[-1]]
+
+
+@pytest.mark.parametrize("kind", ["cache", "batch", "paged", "q4"])
+def test_memory_is_zeroed_before_its_first_use(kind):
+    """Work of the caller's on the default stream, which the zeroing of a new
+    cache runs behind, while the model's own stream is free."""
+    import torch
+    m, ids = Model.from_bytes(_file()), synth.prompt_ids(2048, 40, seed=3)
+
+    def run():
+        if kind == "cache":
+            kv = m.kv_cache(128)
+            m.prefill(ids, kv, last_row_only=True)
+            torch.cuda.synchronize()
+            return kv, m.decode_step(9, kv)
+        kb = m.kv_batch(2, 128, 8 if kind in ("paged", "q4") else 0, 4 if kind == "q4" else 16)
+        kb.prefill(1, ids, True)
+        token = kb.sample([Sampler(1.0, 20, 0.9)], [0.7])[0][0]
+        torch.cuda.synchronize()
+        return kb, kb.decode_step_seqs([1], [9])[0][0], token
+
+    want = run()
+    torch.cuda._sleep(int(4e8))  # about 0.2 s
+    got = run()
+    assert np.all(np.abs(got[1] - want[1]) <= 2e-2 + 1e-2 * np.abs(want[1])), float(np.abs(got[1] - want[1]).max())
+    assert got[2:] == want[2:]
