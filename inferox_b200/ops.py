@@ -346,6 +346,8 @@ def kv4_attention(q, pages, table, kv_len, n_kv_heads: int, q_start=None, scale=
         os = _rows("kv4_attention", out)[3]
     if workspace is None:
         workspace = torch.empty(_workspace_bytes(h, n_kv_heads, d), dtype=torch.uint8, device=q.device)
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise IfxError(24, "kv4_attention: workspace must be a contiguous uint8 tensor")
     dev = _dev(q, pages, table, kv_len, out, workspace) if q_start is None else _dev(
         q, pages, table, kv_len, out, workspace, q_start)
     _call(dev, "kv4_attention", lib.ifx_op_kv4_attention, _TYPES[q.dtype], q.data_ptr(), qs, rows, pages.data_ptr(),

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import serve_rule as SR
-from inferox_b200 import ops
+from inferox_b200 import IfxError, ops
 from test_gpu_serve_ops import cuda, filled, i32
 
 pytestmark = pytest.mark.gpu
@@ -174,3 +174,16 @@ def test_extend_of_impossible_pages_names_no_slot(page):
     r = ops.pages_extend(i32([5, 64]), add, i32([[(1 << 25) - 1, -1], [0, -1]]), i32([4, 3]), i32([2]), 6)
     last = 64 * ((1 << 25) - 1)
     assert r.slots.tolist() == [last + 5, last + 6, last + 7, 192, 193, -1]
+
+
+# -------------------------------------------------------------- refusals
+def test_attention_refuses_a_workspace_that_is_not_its_bytes():
+    """One byte expanded, every other byte, or another type: the count of the
+    elements says nothing of the memory behind them."""
+    H, G, hd = 8, 2, 64
+    pages, q = ops.kv4_pages(2, G, hd), torch.zeros(2, H, hd, device=DEV)
+    ws = ops.kv4_workspace(H, G, hd)
+    for bad in (ws[:1].expand(ws.numel()), torch.cat([ws, ws])[::2], ws.view(torch.float32), ws.view(torch.int8)):
+        with pytest.raises(IfxError, match="InvalidArgument"):
+            ops.kv4_attention(q, pages, i32([[0], [1]]), i32([1, 1]), G, workspace=bad)
+    ops.kv4_attention(q, pages, i32([[0], [1]]), i32([1, 1]), G, workspace=ws)
