@@ -365,11 +365,14 @@ def kv4_workspace(n_heads: int, n_kv_heads: int, head_dim: int, device="cuda") -
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """The next token of every row of logits [rows, n] (float32), by
     Sampler::sample's rule with min-p beside its filters and the uniform draws
-    u [rows] given: (tokens int32 [rows], logprobs float32 [rows]). Settings
-    are tensors [rows] or one value for all rows. temperature <= 0 is greedy;
-    a row whose logits are all masked (-inf, NaN) gives token -1."""
+    u [rows] given, a tensor: (tokens int32 [rows], logprobs float32 [rows]).
+    Settings are tensors [rows] or one value for all rows. A temperature that
+    is not above 0 is greedy; a row whose logits are all masked (-inf, NaN)
+    gives token -1."""
     if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise IfxError(24, "sample_rows: logits must be float32 [rows, n] with contiguous rows")
+    if not isinstance(u, torch.Tensor):  # (one number would be every row's)
+        raise IfxError(24, "sample_rows: u is a float32 tensor, one draw per row")
     rows, n = logits.shape
     at = []
     for x, dt in ((u, torch.float32), (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32),

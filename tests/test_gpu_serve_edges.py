@@ -187,3 +187,12 @@ def test_attention_refuses_a_workspace_that_is_not_its_bytes():
         with pytest.raises(IfxError, match="InvalidArgument"):
             ops.kv4_attention(q, pages, i32([[0], [1]]), i32([1, 1]), G, workspace=bad)
     ops.kv4_attention(q, pages, i32([[0], [1]]), i32([1, 1]), G, workspace=ws)
+
+
+def test_sample_refuses_one_draw_for_all_rows():
+    z = torch.randn(4, 50, device=DEV)
+    for u in (0.5, 1, np.float32(0.5), [0.1, 0.2, 0.3, 0.4]):
+        with pytest.raises(IfxError, match="InvalidArgument"):
+            ops.sample_rows(z, u)
+    with pytest.raises(IfxError, match="Shape"):
+        ops.sample_rows(z, torch.rand(1, device=DEV))
