@@ -471,14 +471,15 @@ ifx_status ifx_op_kv4_attention(int type, const void *q, size_t q_stride,
  * top_p[r] of the whole row's mass (1: all), and of these the ones with
  * w_i >= min_p[r] (0: all). Drawn is the first kept token at which the kept
  * mass so far exceeds u[r] of the kept mass; when no filter is on, in index
- * order. temperature[r] <= 0 takes the largest logit (the last index among
+ * order. A temperature that is not above 0 (NaN among them) takes the largest logit (the last index among
  * equal ones, as argmax). NaN counts as minus infinity, a masked token; a
  * row without any other gives token -1 and logprob -inf. NULL settings:
  * temperature 1, no filter. logprob (nullable): the logarithm of the drawn
  * token's share of the kept mass (0 when greedy). Masses are summed as
  * 64-bit integers (weights to 2^-45 for 128256 tokens, to 2^-50 for 2048 and
- * below), so the result does not depend on the order of additions. Settings
- * that are NaN are off. */
+ * below), so the result does not depend on the order of additions. A top_p or
+ * min_p that is NaN is off; a u outside [0, 1) counts as its nearer end, NaN
+ * as 0. */
 #define IFX_SAMPLE_ROWS_MAX (1 << 24)
 ifx_status ifx_op_sample_rows(const float *logits, size_t stride, size_t rows,
                               size_t n, const float *u,

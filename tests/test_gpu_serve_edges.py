@@ -196,3 +196,16 @@ def test_sample_refuses_one_draw_for_all_rows():
             ops.sample_rows(z, u)
     with pytest.raises(IfxError, match="Shape"):
         ops.sample_rows(z, torch.rand(1, device=DEV))
+
+
+def test_sample_settings_that_are_nan():
+    """NaN temperature: greedy; NaN top_p or min_p: off; NaN u: 0, and u beyond
+    its range at its ends."""
+    z, nan = torch.randn(6, 3000, device=DEV), float("nan")
+    u = torch.rand(6, device=DEV)
+    assert ops.sample_rows(z, u, nan, 5, 0.5)[0].tolist() == z.argmax(1).tolist()
+    for got, want in (((u, 0.8, 40, nan, nan), (u, 0.8, 40)), ((u, 0.8, 0, nan, nan), (u, 0.8)),
+                      ((u * nan, 0.8, 40), (u * 0, 0.8, 40)), ((u - 7, 0.8), (u * 0, 0.8)),
+                      ((u + 7, 0.8, 0, 0.9), (u * 0 + 1 - 2 ** -24, 0.8, 0, 0.9))):
+        a, b = ops.sample_rows(z, *got), ops.sample_rows(z, *want)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
