@@ -381,9 +381,10 @@ ifx_status ifx_op_sample_u_static(const float *logits_dev, size_t n,
  * slot is -1, lens_out = lens, n_free_out = n_free and q_start 0:
  * 1 too few free pages, 2 a sequence longer than max_pages pages (with its new
  * rows or without), 3 more than max_tokens rows. Lengths and counts below 0
- * are 0; a page number that no 32-bit slot can name gives slot -1. Inputs and outputs do not overlap (lens_out may not
- * be lens, nor n_free_out n_free: swap them from step to step); free_pages
- * [n_pages] is not written. At most IFX_PAGES_MAX_SEQS sequences. */
+ * are 0; a page number that no 32-bit slot can name gives slot -1. Inputs and
+ * outputs do not overlap (lens_out may not be lens, nor n_free_out n_free:
+ * swap them from step to step); free_pages [n_pages] is not written. At most
+ * IFX_PAGES_MAX_SEQS sequences. */
 ifx_status ifx_op_pages_extend(const int32_t *lens, const int32_t *add,
                                size_t n_seqs, int32_t *table, size_t max_pages,
                                const int32_t *free_pages, size_t n_pages,
@@ -445,9 +446,11 @@ ifx_status ifx_op_kv4_load(int type, const void *pages, size_t n_pages,
  * query rows per kv head a query enters the products with 22 bits below its
  * head's largest value, and a probability times a value's scale to 2^-20 of
  * the largest such term of a page in the same block of 32 dimensions; with
- * many, queries and probabilities have 22 bits each, and a block whose values
- * are below 2^-19 of the page's largest loses bits. Equal calls repeat bit for
- * bit; a row's last bits may change with the other rows of its call.
+ * many, queries and probabilities have 22 bits each (a probability down to
+ * 2^-35 of the row's largest), and a block whose values are below 2^-19 of the
+ * page's largest loses bits. Equal calls repeat bit for bit; a row's last bits
+ * may change with the other rows of its call. A kv_len beyond the table's
+ * max_pages pages counts as their end.
  * ws: scratch of at least ifx_kv4_attention_workspace bytes, 256-byte
  * aligned, any contents, for one call at a time. */
 size_t ifx_kv4_attention_workspace(size_t n_heads, size_t n_kv_heads,

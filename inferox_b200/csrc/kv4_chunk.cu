@@ -7,8 +7,10 @@
 //   scores: S = q_lo k_hi + q_hi k_lo + q_hi k_hi   (128 x 64 x head_dim)
 //   output: O = p_lo v_hi + p_hi v_lo + p_hi v_hi   (128 x head_dim x 64)
 // with a running maximum and sum per query row. All operands are f16 planes: a
-// value's rounding to f16 and the rounded remainder, 22 bits together; keys
-// and values, four bits times a scale of 11, are exact in two. S and O are f32
+// value's rounding to f16 and the rounded remainder, 22 bits together (of a
+// probability down to 2^-35 of the row's largest so far); keys and values, four
+// bits times a scale of 11, are exact in two down to 2^-19 of their page's
+// largest. O goes over to every page's exponent, by powers of two in f32. S and O are f32
 // in tensor memory and start from zero for every page; O is read back and
 // added in f32, since the tensor cores cut their sums off instead of rounding
 // them (40 pages summed there came out 4.8e-6 off, this way 4e-7).
@@ -27,8 +29,8 @@
 // and its planes 230, unpacking 200, output 32), issued at 57% of the rate;
 // the tensor cores are busy 24% of the time (twelve 128 x 64 x 16 products each
 // way, at full rate). 128 rows of 4 sequences, 32 heads on 8, 2600 keys: heads
-// of 64 74 us (144 TFLOP/s of the two plain products), of 128 119 us, of 256
-// 205 us; the same with m16n8k16 products on 64 rows took 122, 226 and 659.
+// of 64 76 us (140 TFLOP/s of the two plain products), of 128 122 us, of 256
+// 209 us; the same with m16n8k16 products on 64 rows took 122, 226 and 659.
 #include <algorithm>
 
 #include "kv4_attention.cuh"
@@ -678,10 +680,10 @@ ifx_status run_tc(const Kv4AttnArgs &a, cudaStream_t st) {
 
 // 128 query rows a tile pay from 64 columns (query rows of a kv head) on, where
 // there is work enough for the longer way to the first product. 16 sequences,
-// 2600 keys, heads of 64 and 128: 48 columns 72 and 115 us against 71 and 108 of
-// kv4_attention.cu, 64 columns 73 and 116 against 88 and 135, 96 columns 75 and
-// 119 against 123 and 190. One sequence, 8 kv heads: 256 columns of 64 37 us
-// against 35, of 128 40 against 49; 512 columns of 64 39 against 53, over 128
+// 2600 keys, heads of 64 and 128: 48 columns 73 and 119 us against 73 and 112 of
+// kv4_attention.cu, 64 columns 73 and 120 against 90 and 141, 96 columns 75 and
+// 122 against 128 and 200. One sequence, 8 kv heads: 256 columns of 64 37 us
+// against 36, of 128 41 against 50; 512 columns of 64 39 against 54, over 128
 // keys 15 against 17.
 bool kv4_chunks_take(const Kv4AttnArgs &a) {
   const int64_t columns = kv4_columns(a);

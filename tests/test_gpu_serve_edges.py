@@ -147,6 +147,17 @@ def test_attention_windows_longer_than_the_cache(H, G, hd, ql, window):
     close(ops.kv4_attention(*args, **kw, window=window), ref, lim)
 
 
+@pytest.mark.parametrize("ql", [1, 128])
+def test_attention_length_beyond_the_table_counts_as_its_end(ql):
+    H, G, hd = 8, 4, 64
+    rng = np.random.default_rng(2)
+    pages, table, _, _ = filled(rng, [128, 128, 128, 128], G, hd)
+    q, start = cuda(rng.standard_normal((4 * ql, H, hd)).astype(np.float32)), i32(ql * np.arange(5))
+    at = i32(table[:, :2])
+    want = ops.kv4_attention(q, pages, at, i32([128] * 4), G, q_start=start)
+    assert torch.equal(want, ops.kv4_attention(q, pages, at, i32([129, 128, 5000, 2 ** 31 - 1]), G, q_start=start))
+
+
 # ----------------------------------------------------------------- pages
 @pytest.mark.parametrize("lens,add", [([300, 5], [0, 1]), ([257], [0]), ([2 ** 31 - 1, 0], [0, 0]), ([2 ** 31 - 1], [2 ** 31 - 1])])
 def test_extend_refuses_lengths_beyond_the_table(lens, add):
